@@ -8,6 +8,7 @@ for this path (names, argument meaning, error behaviour):
     GeLUMLP.forward(x)                  src/model/mlp.rs:35-41
     Gemma4MoeBlock.forward(x)           src/model/moe.rs:315-470
     KVCache.update_and_fetch(k, v)      src/cache.rs:266-310   (see kv.py)
+    PagedKVCache                        pages for many sequences; no counterpart (see paged.py)
     Gemma4DecoderLayer.forward(x, ...)  src/model/mod.rs:67-119  (see model.py)
     Gemma4Model.decode_step()           src/model/mod.rs:135-363
     ExpertParallelMoeBlock.forward(x)   moe.rs:315-470 with experts split over GPUs (see ep.py)
@@ -154,6 +155,18 @@ SIGNATURES = {
     "fmoe_attn_decode": (_I, [ctypes.POINTER(KvCacheC), _P, _I, _I64, _P, _F, _P, _P, _SZ, _P]),
     "fmoe_attn_decode_sparse_v": (_I, [ctypes.POINTER(KvCacheC), _P, _I, _I64, _F, _F, _P, _P]),
     "fmoe_turbo_round_trip": (_I, [_P, _I64, _I, _I, _P, _P]),
+    "fmoe_paged_bytes": (_SZ, [_P]),
+    "fmoe_paged_workspace_bytes": (_SZ, [_P]),
+    "fmoe_paged_reserve": (_I, [_P, _P, _P, _I, _P, _P, _SZ, _P]),
+    "fmoe_paged_fork": (_I, [_P, _P, _P, _I, _P, _SZ, _P]),
+    "fmoe_paged_free": (_I, [_P, _P, _I, _P]),
+    "fmoe_paged_trim": (_I, [_P, _P, _I, _I, _I, _P]),
+    "fmoe_paged_compact": (_I, [_P, _P, _P, _SZ, _P]),
+    "fmoe_paged_copy": (_I, [_P, _P, _P, _I, _P]),
+    "fmoe_paged_append": (_I, [_P, _I, _P, _I64, _P, _I64, _P, _P]),
+    "fmoe_paged_append_qkv": (_I, [_P, _I, _P, _I64, _I, _P, _I64, _P, _I64, _P, _P, _P, _P]),
+    "fmoe_paged_attend_workspace_bytes": (_SZ, [_P, _I, ctypes.c_int32, _I64, ctypes.c_int32]),
+    "fmoe_paged_attend": (_I, [_P, _I, _P, _I64, _I, _P, _I, _I, _F, _P, _P, _SZ, _P]),
     "fmoe_decoder_workspace_bytes": (_SZ, [_I64, _P, ctypes.POINTER(KvCacheC)]),
     "fmoe_decoder_layer_forward": (_I, [_P, ctypes.POINTER(KvCacheC), _P, _I64, _I64, _P, _P, _SZ, _P]),
     "fmoe_decoder_layer_prefill_workspace_bytes": (_SZ, [_P, _I64]),
@@ -583,6 +596,7 @@ from .kv import KV_AFFINE, KV_BF16, KVCache, turbo_round_trip  # noqa: E402
 from .model import GEMMA4_26B, Gemma4DecoderLayer, Gemma4Model  # noqa: E402
 from .ep import (FMOE_EP_EXACT, FMOE_EP_FIXED, FMOE_EP_P2P, EPComm, ExpertParallelMoeBlock, PeerLost, PeerWatch,  # noqa: E402
                  shard_range)
+from .paged import PagedBatch, PagedKVCache, QKNormRope  # noqa: E402
 from . import ecb  # noqa: E402
 from .tier import HostExpertTier, TieredMoeBlock  # noqa: E402
 from .sample import Sampler, sample_tokens  # noqa: E402

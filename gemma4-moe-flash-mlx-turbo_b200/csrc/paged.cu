@@ -1,0 +1,754 @@
+// Pages of a cache for many sequences: room for new positions, forks that share
+// full pages, freeing, compaction; and the passes that store a step's rows.
+//
+// Pages are handed out lowest id first, in the order of the call's sequences,
+// so a call's result depends on the state alone, never on the order in which
+// threads arrive: one CTA finds the free pages by a scan over the counts and
+// gives the k-th free page to the k-th request.  What moves bytes (the copies
+// of part-filled or compacted pages) runs in a second kernel over all SMs,
+// from the list that the first one wrote.
+#include <algorithm>
+#include <cmath>
+#include "paged.cuh"
+#include "stage.cuh"
+#include "kvrow.cuh"
+#include "rowops.cuh"
+
+namespace fmoe {
+namespace pg {
+
+constexpr int kPlan = 1024;  // threads of the planning CTA
+
+struct Ws {
+  int32_t* count;  // [4] 0: moves in the list
+  int32_t* src;    // [max(num_pages, max_seqs)]
+  int32_t* dst;
+  int32_t* map;    // [num_pages] where a page went (compact)
+  int32_t* claim;  // [max_seqs] lowest pair that names the row as its child (fork)
+  int32_t* parent; // [max_seqs] 1: some pair's parent
+  int32_t* got;    // [max_seqs] per pair: the page for its part-filled block, -1 none needed, -2 refused
+};
+
+// Exclusive prefix sum of v over the CTA; *total receives the sum.
+__device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // sh is reused across calls
+  if (lane == 31) sh[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int w = sh[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    sh[lane] = w;
+  }
+  __syncthreads();
+  *total = sh[31];
+  return (warp ? sh[warp - 1] : 0) + x - v;
+}
+
+// The ids in [from, to) whose count is zero (FREE) or not, in order, to
+// list[0 .. want); returns how many there are, at most want.  The counts were
+// changed by atomics of this CTA, so they are read from L2.
+template <bool FREE>
+__device__ int find_pages(const int32_t* refs, int from, int to, int want, int32_t* list, int* sh) {
+  int found = 0;
+  for (int a = from; a < to && found < want; a += 4 * kPlan) {
+    const int i = a + 4 * threadIdx.x;
+    bool hit[4];
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      hit[u] = i + u < to && (__ldcg(refs + i + u) == 0) == FREE;
+      n += hit[u];
+    }
+    int total;
+    int at = found + block_scan(n, sh, &total);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (hit[u]) {
+        if (at < want) list[at] = i + u;
+        ++at;
+      }
+    found += total;
+  }
+  __syncthreads();
+  return min(found, want);
+}
+
+__device__ __forceinline__ int blocks_of(const PagedDev& c, int len) { return (len + c.ps - 1) >> c.log_ps; }
+
+__global__ void __launch_bounds__(kPlan) paged_reserve_kernel(PagedDev c, const int32_t* __restrict__ seqs,
+                                                              const int32_t* __restrict__ counts, int n,
+                                                              int32_t* __restrict__ kv_len, Ws w) {
+  __shared__ int sh[32];
+  __shared__ unsigned long long want_sh;
+  const int tid = threadIdx.x, lane = tid & 31;
+  // pages that sequence i asks for (at most one more than there are: a scan's
+  // sum over the CTA then fits 32 bits); -1: it cannot have them, whatever is free
+  auto asks = [&](int i, int& seq, int& len) {
+    seq = seqs[i];
+    if (seq < 0 || seq >= c.max_seqs) return -1;
+    len = c.lens[seq];
+    const int add = counts[i];
+    if (len < 0 || add < 0 || (int64_t)len + add > (int64_t)c.max_blocks * c.ps) return -1;
+    return min(blocks_of(c, len + add) - blocks_of(c, len), c.num_pages + 1);
+  };
+  if (tid == 0) want_sh = 0;
+  __syncthreads();
+  unsigned long long sum = 0;
+  int seq = 0, len = 0;
+  for (int i = tid; i < n; i += kPlan) sum += max(0, asks(i, seq, len));
+  if (sum) atomicAdd(&want_sh, sum);
+  __syncthreads();
+  const int want = (int)min(want_sh, (unsigned long long)c.num_pages);
+  const int free_n = find_pages<true>(c.refs, 0, c.num_pages, want, w.src, sh);
+  int64_t before = 0;  // pages asked for by the sequences of earlier rounds
+  for (int i0 = 0; i0 < n; i0 += kPlan) {
+    const int i = i0 + tid;
+    const int need = i < n ? asks(i, seq, len) : 0;
+    int total;
+    const int64_t at = before + block_scan(max(need, 0), sh, &total);
+    const bool ok = need == 0 || (need > 0 && at + need <= free_n);
+    for (int l = 0; l < 32; ++l) {  // the warp hands out each of its sequences' pages together
+      const int k1 = __shfl_sync(0xffffffffu, ok ? need : 0, l);
+      if (k1 == 0) continue;
+      const int a1 = (int)__shfl_sync(0xffffffffu, ok ? (int)at : 0, l);
+      const int64_t t1 = (int64_t)__shfl_sync(0xffffffffu, seq, l) * c.max_blocks +
+                         blocks_of(c, __shfl_sync(0xffffffffu, len, l));
+      for (int k = lane; k < k1; k += 32) {
+        const int p = w.src[a1 + k];
+        c.table[t1 + k] = p;
+        c.refs[p] = 1;
+      }
+    }
+    if (i < n) {
+      if (ok) {
+        c.lens[seq] = len + counts[i];
+        kv_len[i] = len + counts[i];
+      } else {
+        kv_len[i] = -1;
+        atomicAdd(c.refused, 1);
+      }
+    }
+    before += total;
+  }
+}
+
+// fork, first half: what children held is let go, pairs are checked, and the
+// part-filled last blocks get their pages.
+__global__ void __launch_bounds__(kPlan) paged_fork_plan_kernel(PagedDev c, const int32_t* __restrict__ parents,
+                                                                const int32_t* __restrict__ children, int n, Ws w) {
+  __shared__ int sh[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto row = [&](int s) { return s >= 0 && s < c.max_seqs; };
+  for (int i = tid; i < c.max_seqs; i += kPlan) {
+    w.claim[i] = INT32_MAX;
+    w.parent[i] = 0;
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kPlan) {
+    if (row(parents[i])) w.parent[parents[i]] = 1;
+    if (row(children[i])) atomicMin(&w.claim[children[i]], i);
+  }
+  __syncthreads();
+  auto valid = [&](int i) {
+    const int p = parents[i], d = children[i];
+    return row(p) && row(d) && __ldcg(&w.claim[d]) == i && !__ldcg(&w.parent[d]);
+  };
+  for (int i = warp; i < n; i += kPlan / 32) {
+    if (!valid(i)) continue;
+    int32_t* t = c.table + (int64_t)children[i] * c.max_blocks;
+    for (int b = lane; b < c.max_blocks; b += 32) {
+      const int p = t[b];
+      if (p >= 0) {
+        if (p < c.num_pages) atomicSub(&c.refs[p], 1);
+        t[b] = -1;
+      }
+    }
+    if (lane == 0) c.lens[children[i]] = 0;
+  }
+  __syncthreads();
+  const int free_n = find_pages<true>(c.refs, 0, c.num_pages, min(n, c.num_pages), w.dst, sh);
+  int before = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlan) {
+    const int i = i0 + tid;
+    int last = -1;  // page of the part-filled block
+    bool ok = false;
+    if (i < n && (ok = valid(i))) {
+      const int len = c.lens[parents[i]];
+      if (len & (c.ps - 1)) last = page_of(c, parents[i], len >> c.log_ps);
+    }
+    int total;
+    const int at = before + block_scan(last >= 0, sh, &total);
+    before += total;
+    if (i < n) {
+      const bool have = ok && (last < 0 || at < free_n);
+      w.got[i] = !have ? -2 : last < 0 ? -1 : w.dst[at];
+      if (last >= 0 && have) {
+        w.src[at] = last;
+        c.refs[w.dst[at]] = 1;  // its child's row holds it
+      }
+      if (!have) atomicAdd(c.refused, 1);
+    }
+  }
+  if (tid == 0) w.count[0] = min(before, free_n);
+}
+
+// Moves listed pages of every layer: a unit is 16 KB of one page in one layer;
+// each thread has four 16-byte loads in flight before its first store.
+__device__ __forceinline__ void move_pages(const PagedDev& c, const int32_t* src, const int32_t* dst, int moves, int cta,
+                                           int ctas) {
+  constexpr int kUnit = 16384, kVec = kUnit / 16 / 256;
+  const int per = (int)((c.page + kUnit - 1) / kUnit);
+  const int64_t units = (int64_t)moves * c.layers * per;
+  for (int64_t u = cta; u < units; u += ctas) {
+    const int part = (int)(u % per);
+    const int64_t q = u / per;
+    const int layer = (int)(q % c.layers), m = (int)(q / c.layers);
+    const int s = src[m], d = dst[m];
+    if (s < 0 || d < 0 || s >= c.num_pages || d >= c.num_pages) continue;
+    const uint8_t* a = c.pages + layer * c.layer + s * c.page + (int64_t)part * kUnit;
+    uint8_t* b = c.pages + layer * c.layer + d * c.page + (int64_t)part * kUnit;
+    const int left = (int)min((int64_t)kUnit, c.page - (int64_t)part * kUnit);
+    uint4 v[kVec];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      const int o = (k * 256 + (int)threadIdx.x) * 16;
+      if (o < left) v[k] = ld_u4(a + o);
+    }
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) {
+      const int o = (k * 256 + (int)threadIdx.x) * 16;
+      if (o < left) *reinterpret_cast<uint4*>(b + o) = v[k];
+    }
+  }
+}
+
+// fork, second half: the children's rows, the counts of shared pages, the copies.
+__global__ void __launch_bounds__(256) paged_fork_apply_kernel(PagedDev c, const int32_t* __restrict__ parents,
+                                                               const int32_t* __restrict__ children, int n, Ws w) {
+  const int lane = threadIdx.x & 31;
+  const int warps = (gridDim.x * blockDim.x) >> 5;
+  for (int i = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < n; i += warps) {
+    const int got = w.got[i];
+    if (got == -2) continue;
+    const int32_t* from = c.table + (int64_t)parents[i] * c.max_blocks;
+    int32_t* to = c.table + (int64_t)children[i] * c.max_blocks;
+    const int len = c.lens[parents[i]];
+    const int nb = min(blocks_of(c, len), c.max_blocks);
+    for (int b = lane; b < nb; b += 32) {
+      int p = from[b];
+      if (got >= 0 && b == nb - 1)
+        p = got;
+      else if (p >= 0 && p < c.num_pages)
+        atomicAdd(&c.refs[p], 1);
+      to[b] = p;
+    }
+    if (lane == 0) c.lens[children[i]] = len;
+  }
+  move_pages(c, w.src, w.dst, w.count[0], blockIdx.x, gridDim.x);
+}
+
+// free (window 0) and trim: a warp per sequence lets go of the pages of blocks
+// [b0, b1): all, or those that end at or before the window's first position
+// and begin at or after the first `sinks`.
+__global__ void __launch_bounds__(256) paged_release_kernel(PagedDev c, const int32_t* __restrict__ seqs, int n,
+                                                            int window, int sinks) {
+  const int i = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  if (i >= n) return;
+  const int s = seqs[i];
+  if (s < 0 || s >= c.max_seqs) return;
+  int b0 = 0, b1 = c.max_blocks;
+  if (window > 0) {
+    // the next query is at position len and sees j > len - window
+    const int64_t low = (int64_t)c.lens[s] - window + 1;
+    b0 = blocks_of(c, sinks);
+    b1 = low > 0 ? (int)min((int64_t)c.max_blocks, low >> c.log_ps) : 0;
+  } else if (lane == 0) {
+    c.lens[s] = 0;
+  }
+  int32_t* t = c.table + (int64_t)s * c.max_blocks;
+  for (int b = b0 + lane; b < b1; b += 32) {
+    const int p = t[b];
+    if (p < 0) continue;
+    if (p < c.num_pages) atomicSub(&c.refs[p], 1);
+    t[b] = -1;
+  }
+}
+
+// compact, first half: which page goes where, and the counts after it.
+__global__ void __launch_bounds__(kPlan) paged_compact_plan_kernel(PagedDev c, int32_t* __restrict__ live, Ws w) {
+  __shared__ int sh[32], n_sh;
+  const int tid = threadIdx.x;
+  if (tid == 0) n_sh = 0;
+  __syncthreads();
+  int mine = 0;
+  for (int i = tid; i < c.num_pages; i += kPlan) {
+    mine += c.refs[i] != 0;
+    w.map[i] = i;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if ((tid & 31) == 0) atomicAdd(&n_sh, mine);
+  __syncthreads();
+  const int n = n_sh;
+  const int holes = find_pages<true>(c.refs, 0, n, n, w.dst, sh);
+  find_pages<false>(c.refs, n, c.num_pages, holes, w.src, sh);  // as many as there are holes
+  for (int k = tid; k < holes; k += kPlan) {
+    const int s = w.src[k], d = w.dst[k];
+    w.map[s] = d;
+    c.refs[d] = c.refs[s];
+    c.refs[s] = 0;
+  }
+  if (tid == 0) {
+    w.count[0] = holes;
+    *live = n;
+  }
+}
+
+__global__ void __launch_bounds__(256) paged_compact_apply_kernel(PagedDev c, Ws w) {
+  const int moves = w.count[0];
+  if (!moves) return;
+  const int64_t entries = (int64_t)c.max_seqs * c.max_blocks;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < entries; i += (int64_t)gridDim.x * blockDim.x) {
+    const int p = c.table[i];
+    if (p >= 0 && p < c.num_pages) {
+      const int q = w.map[p];
+      if (q != p) c.table[i] = q;
+    }
+  }
+  move_pages(c, w.src, w.dst, moves, blockIdx.x, gridDim.x);
+}
+
+__global__ void __launch_bounds__(256) paged_copy_kernel(PagedDev c, const int32_t* __restrict__ src,
+                                                         const int32_t* __restrict__ dst, int n) {
+  move_pages(c, src, dst, n, blockIdx.x, gridDim.x);
+}
+
+// ---------------------------------------------------------------------------
+// storing a step's rows
+
+// The sequence of row t (n: none): how many sequences end at or before it.
+__device__ __forceinline__ int seq_of_row(const BatchDev& b, int64_t t) {
+  int count = 0;
+  for (int i = 0; i < b.n; i += blockDim.x) {
+    const int k = i + threadIdx.x;
+    count += __syncthreads_count(k < b.n && __ldg(b.q_start + k + 1) <= t);
+  }
+  return count;
+}
+
+// Lane l's values l * P .. of a row, quantised in groups of 64 into the page
+// format's words (octet o, group g at word o * (D / 64) + g) and pairs.
+template <int P>
+__device__ __forceinline__ void store_q4(const float (&v)[P], int lane, uint32_t* words, uint32_t* pairs) {
+  constexpr int LG = 64 / P, NG = P / 2;  // lanes of a group, groups of a row
+  float mn = v[0], mx = v[0];
+#pragma unroll
+  for (int i = 1; i < P; ++i) {
+    mn = fminf(mn, v[i]);
+    mx = fmaxf(mx, v[i]);
+  }
+#pragma unroll
+  for (int o = 1; o < LG; o <<= 1) {
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  float scale = __fdiv_rn(__fsub_rn(mx, mn), 15.0f);
+  if (!(scale >= 1e-7f)) scale = 1e-7f;
+  const bf16 sb = __float2bfloat16_rn(scale), bb = __float2bfloat16_rn(mn);
+  const float s = bf2f(sb), b = bf2f(bb);
+  const int g = lane / LG;
+#pragma unroll
+  for (int o = 0; o < P / 8; ++o) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float q = rintf(__fdiv_rn(__fsub_rn(v[8 * o + i], b), s));
+      q = fminf(fmaxf(q, 0.0f), 15.0f);
+      w |= (uint32_t)q << (4 * ((i >> 1) + 4 * (i & 1)));
+    }
+    words[((lane % LG) * (P / 8) + o) * NG + g] = w;
+  }
+  if (lane % LG == 0) {
+    const __nv_bfloat162 sp = __halves2bfloat162(sb, bb);
+    pairs[g] = *reinterpret_cast<const uint32_t*>(&sp);
+  }
+}
+
+template <int P>
+__device__ __forceinline__ void store_page_row(const PagedDev& c, int layer, int page, int slot, int h, int which,
+                                               const float (&v)[P], int lane) {
+  constexpr int D = 32 * P;
+  uint8_t* blk = page_block(c, layer, page, h, which);
+  if (c.bits == 16)
+    store_row_bf16<P>(reinterpret_cast<bf16*>(blk) + (int64_t)slot * D, lane, v);
+  else
+    store_q4<P>(v, lane, reinterpret_cast<uint32_t*>(blk + slot * (D / 2)),
+                reinterpret_cast<uint32_t*>(blk + c.ps * (D / 2) + slot * (D / 16)));
+}
+
+struct RowsIn {
+  const bf16 *q, *k, *v, *qn, *kn;
+  int64_t qs, ks, vs;  // row strides, values
+  int Hq, rope;
+  float eps;
+  double l2t;  // log2(theta)
+  bf16* q_out;
+};
+
+// One CTA per row of the step; a warp takes heads of it.  NORM: norms and
+// rotation (append_qkv); otherwise k and v as they are.
+template <int P, bool NORM>
+__global__ void __launch_bounds__(256) paged_rows_kernel(PagedDev c, int layer, BatchDev b, RowsIn a) {
+  constexpr int D = 32 * P;
+  __shared__ float tcos[NORM ? D / 2 : 1], tsin[NORM ? D / 2 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t = blockIdx.x;
+  const int i = seq_of_row(b, t);
+  if (i >= b.n) return;
+  const int len = b.kv_len[i], pos = len - b.q_start[i + 1] + (int)t;
+  const int half = a.rope / 2;
+  if (NORM) {
+    // angle in turns = pos * theta^(-2j / rope) / 2 pi, reduced in 64 bits: a
+    // position of 10^5 times a 32-bit rate is off by a hundredth of a radian
+    for (int j = threadIdx.x; j < half; j += blockDim.x) {
+      const double turns = pos * (exp2(-(double)(2 * j) / a.rope * a.l2t) * 0.15915494309189535);
+      sincospif(2.0f * (float)(turns - rint(turns)), &tsin[j], &tcos[j]);
+    }
+    __syncthreads();
+  }
+  const int page = pos >= 0 && pos < len ? page_of(c, b.seqs[i], pos >> c.log_ps) : -1;
+  const int slot = pos & (c.ps - 1);
+  for (int hh = warp; hh < (NORM ? a.Hq : 0) + 2 * c.Hkv; hh += blockDim.x / 32) {
+    float x[P];
+    const int h = NORM ? hh - a.Hq : hh;
+    const bool is_v = h >= c.Hkv;
+    const bf16* src = h < 0 ? a.q + t * a.qs + (int64_t)hh * D
+                      : is_v && a.v ? a.v + t * a.vs + (int64_t)(h - c.Hkv) * D
+                                    : a.k + t * a.ks + (int64_t)(is_v ? h - c.Hkv : h) * D;
+    if (h >= 0 && page < 0) continue;
+    load_row_f32<P>(src, lane, x);
+    if (NORM) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < P; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = rsqrtf(ss / (float)D + a.eps);
+      if (is_v) {
+#pragma unroll
+        for (int e = 0; e < P; ++e) x[e] *= r;
+      } else {
+        float wv[P];
+        load_row_f32<P>(h < 0 ? a.qn : a.kn, lane, wv);
+#pragma unroll
+        for (int e = 0; e < P; ++e) x[e] *= r * wv[e];
+        const int ofs = half / P;
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const float up = __shfl_down_sync(0xffffffffu, x[e], ofs & 31);
+          const float dn = __shfl_up_sync(0xffffffffu, x[e], ofs & 31);
+          const int d = lane * P + e;
+          if (d < half)
+            x[e] = x[e] * tcos[d] - up * tsin[d];
+          else if (d < 2 * half)
+            x[e] = x[e] * tcos[d - half] + dn * tsin[d - half];
+        }
+      }
+    }
+    if (h < 0)
+      store_row_bf16<P>(a.q_out + (t * a.Hq + hh) * D, lane, x);
+    else
+      store_page_row<P>(c, layer, page, slot, is_v ? h - c.Hkv : h, is_v, x, lane);
+  }
+}
+
+size_t carve(void* base, const PagedDev& c, Ws* w) {
+  Carver k(base);
+  const size_t n = (size_t)std::max(c.num_pages, c.max_seqs);
+  w->count = k.take<int32_t>(4);
+  w->src = k.take<int32_t>(n);
+  w->dst = k.take<int32_t>(n);
+  w->map = k.take<int32_t>(c.num_pages);
+  w->claim = k.take<int32_t>(c.max_seqs);
+  w->parent = k.take<int32_t>(c.max_seqs);
+  w->got = k.take<int32_t>(c.max_seqs);
+  return align_up(k.off, 256);
+}
+
+int to_ws(const PagedDev& c, void* ws, size_t bytes, Ws* w, const char* what) {
+  const size_t need = carve(nullptr, c, w);
+  if (!ws || bytes < need || !aligned(ws, 16))
+    return set_error(FMOE_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, bytes, need);
+  carve(ws, c, w);
+  return FMOE_OK;
+}
+
+// CTAs of a kernel that moves up to `moves` pages: enough to fill the SMs.
+unsigned move_grid(const PagedDev& c, int64_t moves) {
+  const int64_t units = moves * c.layers * ((c.page + 16383) / 16384);
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>(units, 8 * kNumSMs));
+}
+
+int rows_ok(const char* what, const char* name, const void* p, int64_t stride, int64_t width) {
+  if (!p || !aligned(p, 16)) return set_error(FMOE_ERR_ALIGN, "%s: %s null or not 16-byte aligned", what, name);
+  if (stride % 8 || stride < width)
+    return set_error(FMOE_ERR_ALIGN, "%s: %s rows %lld values apart (a multiple of 8, at least %lld)", what, name,
+                     (long long)stride, (long long)width);
+  return FMOE_OK;
+}
+
+int ids_ok(const PagedDev& c, const char* what, int n, const void* a, const void* b) {
+  if (n < 0 || n > c.max_seqs) return set_error(FMOE_ERR_INVALID, "%s: %d sequences of %d", what, n, c.max_seqs);
+  if (n && (!a || !b)) return set_error(FMOE_ERR_INVALID, "%s: null ids", what);
+  return FMOE_OK;
+}
+
+}  // namespace pg
+
+// Checks a cache; need_pages false: its shape only (sizes).
+int paged_to_dev(const fmoe_paged_kv_t* c, PagedDev* d, bool need_pages) {
+  if (!c) return set_error(FMOE_ERR_INVALID, "paged: null cache");
+  if (c->head_dim != 256 && c->head_dim != 512)
+    return set_error(FMOE_ERR_UNSUPPORTED, "paged: head_dim %d (kernels: 256, 512)", c->head_dim);
+  if (c->bits != 16 && c->bits != 4) return set_error(FMOE_ERR_UNSUPPORTED, "paged: bits %d (16, 4)", c->bits);
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+    return set_error(FMOE_ERR_UNSUPPORTED, "paged: page_size %d (16, 32, 64, 128)", c->page_size);
+  if (c->layers < 1 || c->kv_heads < 1 || c->kv_heads > 1024 || c->num_pages < 1 || c->max_seqs < 1 ||
+      c->max_blocks < 1 || c->num_pages > (1 << 21) - 2 || c->max_seqs > (1 << 24) ||
+      c->max_blocks > (1 << 30) / c->page_size)
+    return set_error(FMOE_ERR_INVALID, "paged: layers %d kv_heads %d num_pages %d max_seqs %d max_blocks %d", c->layers,
+                     c->kv_heads, c->num_pages, c->max_seqs, c->max_blocks);
+  if (need_pages) {
+    if (!c->pages || !aligned(c->pages, 128))
+      return set_error(FMOE_ERR_ALIGN, "paged: pages null or not 128-byte aligned");
+    if (!c->table || !c->lens || !c->refs || !c->refused || !aligned(c->table, 4) || !aligned(c->lens, 4) ||
+        !aligned(c->refs, 4) || !aligned(c->refused, 4))
+      return set_error(FMOE_ERR_INVALID, "paged: table, lens, refs or refused null or misaligned");
+  }
+  d->pages = static_cast<uint8_t*>(c->pages);
+  d->table = c->table;
+  d->lens = c->lens;
+  d->refs = c->refs;
+  d->refused = c->refused;
+  d->layers = c->layers;
+  d->Hkv = c->kv_heads;
+  d->D = c->head_dim;
+  d->ps = c->page_size;
+  d->log_ps = c->page_size == 16 ? 4 : c->page_size == 32 ? 5 : c->page_size == 64 ? 6 : 7;
+  d->bits = c->bits;
+  d->num_pages = c->num_pages;
+  d->max_seqs = c->max_seqs;
+  d->max_blocks = c->max_blocks;
+  d->block = (int64_t)d->ps * (d->bits == 16 ? 2 * d->D : d->D / 2 + d->D / 16);
+  d->page = 2 * d->block * d->Hkv;
+  d->layer = d->page * d->num_pages;
+  return FMOE_OK;
+}
+
+int batch_to_dev(const fmoe_paged_batch_t* b, BatchDev* d) {
+  if (!b) return set_error(FMOE_ERR_INVALID, "paged: null batch");
+  if (b->n < 0 || b->tokens < 0 || b->max_new < 0 || b->tokens > INT32_MAX / 2 || b->n > (1 << 20))
+    return set_error(FMOE_ERR_INVALID, "paged: batch of %d sequences, %lld rows, max_new %d", b->n,
+                     (long long)b->tokens, b->max_new);
+  if (b->n && (!b->seqs || !b->q_start || !b->kv_len))
+    return set_error(FMOE_ERR_INVALID, "paged: batch with null seqs, q_start or kv_len");
+  d->seqs = b->seqs;
+  d->q_start = b->q_start;
+  d->kv_len = b->kv_len;
+  d->n = b->n;
+  d->max_new = b->max_new;
+  d->tokens = b->tokens;
+  return FMOE_OK;
+}
+
+template <bool NORM>
+static int launch_rows(const PagedDev& c, int layer, const BatchDev& b, const pg::RowsIn& a, cudaStream_t st) {
+  if (b.tokens == 0 || b.n == 0) return FMOE_OK;
+  ProfScope prof_(NORM ? "paged_rows_kernel<norm>" : "paged_rows_kernel", st);
+  if (c.D == 256)
+    pg::paged_rows_kernel<8, NORM><<<(unsigned)b.tokens, 256, 0, st>>>(c, layer, b, a);
+  else
+    pg::paged_rows_kernel<16, NORM><<<(unsigned)b.tokens, 256, 0, st>>>(c, layer, b, a);
+  return check_launch("paged_rows_kernel");
+}
+
+}  // namespace fmoe
+
+using namespace fmoe;
+using namespace fmoe::pg;
+
+extern "C" {
+
+size_t fmoe_paged_bytes(const fmoe_paged_kv_t* cache) {
+  PagedDev c;
+  return paged_to_dev(cache, &c, false) ? 0 : (size_t)(c.layer * c.layers);
+}
+
+size_t fmoe_paged_workspace_bytes(const fmoe_paged_kv_t* cache) {
+  PagedDev c;
+  Ws w;
+  return paged_to_dev(cache, &c, false) ? 0 : carve(nullptr, c, &w);
+}
+
+int fmoe_paged_reserve(const fmoe_paged_kv_t* cache, const int32_t* seqs, const int32_t* counts, int n,
+                       int32_t* kv_len, void* workspace, size_t workspace_bytes, void* stream) {
+  PagedDev c;
+  Ws w;
+  int rc;
+  if ((rc = paged_to_dev(cache, &c, true)) || (rc = ids_ok(c, "paged_reserve", n, seqs, counts)) ||
+      (rc = to_ws(c, workspace, workspace_bytes, &w, "paged_reserve")))
+    return rc;
+  if (n == 0) return FMOE_OK;
+  if (!kv_len) return set_error(FMOE_ERR_INVALID, "paged_reserve: null kv_len");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope prof_("paged_reserve_kernel", st);
+  paged_reserve_kernel<<<1, kPlan, 0, st>>>(c, seqs, counts, n, kv_len, w);
+  return check_launch("paged_reserve_kernel");
+}
+
+int fmoe_paged_fork(const fmoe_paged_kv_t* cache, const int32_t* parents, const int32_t* children, int n,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  PagedDev c;
+  Ws w;
+  int rc;
+  if ((rc = paged_to_dev(cache, &c, true)) || (rc = ids_ok(c, "paged_fork", n, parents, children)) ||
+      (rc = to_ws(c, workspace, workspace_bytes, &w, "paged_fork")))
+    return rc;
+  if (n == 0) return FMOE_OK;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  {
+    ProfScope prof_("paged_fork_plan_kernel", st);
+    paged_fork_plan_kernel<<<1, kPlan, 0, st>>>(c, parents, children, n, w);
+  }
+  if ((rc = check_launch("paged_fork_plan_kernel"))) return rc;
+  ProfScope prof_("paged_fork_apply_kernel", st);
+  paged_fork_apply_kernel<<<move_grid(c, n), 256, 0, st>>>(c, parents, children, n, w);
+  return check_launch("paged_fork_apply_kernel");
+}
+
+static int release(const char* what, const fmoe_paged_kv_t* cache, const int32_t* seqs, int n, int window, int sinks,
+                   void* stream) {
+  PagedDev c;
+  int rc;
+  if ((rc = paged_to_dev(cache, &c, true)) || (rc = ids_ok(c, what, n, seqs, seqs))) return rc;
+  if (n == 0) return FMOE_OK;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope prof_("paged_release_kernel", st);
+  paged_release_kernel<<<(n + 7) / 8, 256, 0, st>>>(c, seqs, n, window, sinks);
+  return check_launch("paged_release_kernel");
+}
+
+int fmoe_paged_free(const fmoe_paged_kv_t* cache, const int32_t* seqs, int n, void* stream) {
+  return release("paged_free", cache, seqs, n, 0, 0, stream);
+}
+
+int fmoe_paged_trim(const fmoe_paged_kv_t* cache, const int32_t* seqs, int n, int window, int sinks, void* stream) {
+  if (window < 1 || sinks < 0) return set_error(FMOE_ERR_INVALID, "paged_trim: window %d sinks %d", window, sinks);
+  return release("paged_trim", cache, seqs, n, window, std::min(sinks, 1 << 30), stream);
+}
+
+int fmoe_paged_compact(const fmoe_paged_kv_t* cache, int32_t* live, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  PagedDev c;
+  Ws w;
+  int rc;
+  if ((rc = paged_to_dev(cache, &c, true)) || (rc = to_ws(c, workspace, workspace_bytes, &w, "paged_compact")))
+    return rc;
+  if (!live) return set_error(FMOE_ERR_INVALID, "paged_compact: null live");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  {
+    ProfScope prof_("paged_compact_plan_kernel", st);
+    paged_compact_plan_kernel<<<1, kPlan, 0, st>>>(c, live, w);
+  }
+  if ((rc = check_launch("paged_compact_plan_kernel"))) return rc;
+  ProfScope prof_("paged_compact_apply_kernel", st);
+  paged_compact_apply_kernel<<<move_grid(c, c.num_pages), 256, 0, st>>>(c, w);
+  return check_launch("paged_compact_apply_kernel");
+}
+
+int fmoe_paged_copy(const fmoe_paged_kv_t* cache, const int32_t* src, const int32_t* dst, int n, void* stream) {
+  PagedDev c;
+  int rc;
+  if ((rc = paged_to_dev(cache, &c, true))) return rc;
+  if (n < 0 || n > c.num_pages) return set_error(FMOE_ERR_INVALID, "paged_copy: %d pages of %d", n, c.num_pages);
+  if (n == 0) return FMOE_OK;
+  if (!src || !dst) return set_error(FMOE_ERR_INVALID, "paged_copy: null ids");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ProfScope prof_("paged_copy_kernel", st);
+  paged_copy_kernel<<<move_grid(c, n), 256, 0, st>>>(c, src, dst, n);
+  return check_launch("paged_copy_kernel");
+}
+
+int fmoe_paged_append(const fmoe_paged_kv_t* cache, int layer, const void* k, int64_t k_stride, const void* v,
+                      int64_t v_stride, const fmoe_paged_batch_t* batch, void* stream) {
+  PagedDev c;
+  BatchDev b;
+  int rc;
+  if ((rc = paged_to_dev(cache, &c, true)) || (rc = batch_to_dev(batch, &b))) return rc;
+  if (layer < 0 || layer >= c.layers) return set_error(FMOE_ERR_INVALID, "paged_append: layer %d of %d", layer, c.layers);
+  if (b.tokens == 0 || b.n == 0) return FMOE_OK;
+  const int64_t width = (int64_t)c.Hkv * c.D;
+  if ((rc = rows_ok("paged_append", "k", k, k_stride, width)) || (rc = rows_ok("paged_append", "v", v, v_stride, width)))
+    return rc;
+  RowsIn a = {};
+  a.k = static_cast<const bf16*>(k);
+  a.v = static_cast<const bf16*>(v);
+  a.ks = k_stride;
+  a.vs = v_stride;
+  return launch_rows<false>(c, layer, b, a, static_cast<cudaStream_t>(stream));
+}
+
+int fmoe_paged_append_qkv(const fmoe_paged_kv_t* cache, int layer, const void* q, int64_t q_stride, int q_heads,
+                          const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                          const fmoe_paged_batch_t* batch, const fmoe_qk_norm_rope_t* norm, void* q_out, void* stream) {
+  PagedDev c;
+  BatchDev b;
+  int rc;
+  if ((rc = paged_to_dev(cache, &c, true)) || (rc = batch_to_dev(batch, &b))) return rc;
+  if (layer < 0 || layer >= c.layers)
+    return set_error(FMOE_ERR_INVALID, "paged_append_qkv: layer %d of %d", layer, c.layers);
+  if (q_heads < 1 || q_heads > 8192) return set_error(FMOE_ERR_INVALID, "paged_append_qkv: %d query heads", q_heads);
+  if (!norm || !norm->q_norm || !norm->k_norm || !aligned(norm->q_norm, 16) || !aligned(norm->k_norm, 16))
+    return set_error(FMOE_ERR_ALIGN, "paged_append_qkv: norm, q_norm or k_norm null or not 16-byte aligned");
+  if (norm->rope_dims < 0 || norm->rope_dims > c.D || norm->rope_dims % (c.D / 16))
+    return set_error(FMOE_ERR_UNSUPPORTED, "paged_append_qkv: rope_dims %d (a multiple of %d up to %d)",
+                     norm->rope_dims, c.D / 16, c.D);
+  if (!(norm->eps >= 0.f) || (norm->rope_dims && !(norm->rope_theta > 0.f && std::isfinite(norm->rope_theta))))
+    return set_error(FMOE_ERR_INVALID, "paged_append_qkv: eps %g rope_theta %g", (double)norm->eps,
+                     (double)norm->rope_theta);
+  if (b.tokens == 0 || b.n == 0) return FMOE_OK;
+  const int64_t width = (int64_t)c.Hkv * c.D;
+  if ((rc = rows_ok("paged_append_qkv", "q", q, q_stride, (int64_t)q_heads * c.D)) ||
+      (rc = rows_ok("paged_append_qkv", "k", k, k_stride, width)) ||
+      (v && (rc = rows_ok("paged_append_qkv", "v", v, v_stride, width))))
+    return rc;
+  if (!q_out || !aligned(q_out, 16)) return set_error(FMOE_ERR_ALIGN, "paged_append_qkv: q_out null or misaligned");
+  RowsIn a = {};
+  a.q = static_cast<const bf16*>(q);
+  a.k = static_cast<const bf16*>(k);
+  a.v = static_cast<const bf16*>(v);
+  a.qn = static_cast<const bf16*>(norm->q_norm);
+  a.kn = static_cast<const bf16*>(norm->k_norm);
+  a.qs = q_stride;
+  a.ks = k_stride;
+  a.vs = v_stride;
+  a.Hq = q_heads;
+  a.rope = norm->rope_dims;
+  a.eps = norm->eps;
+  a.l2t = norm->rope_dims ? std::log2((double)norm->rope_theta) : 0.0;
+  a.q_out = static_cast<bf16*>(q_out);
+  return launch_rows<true>(c, layer, b, a, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

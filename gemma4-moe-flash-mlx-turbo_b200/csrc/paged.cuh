@@ -1,0 +1,36 @@
+// Device view of a paged KV cache (fmoe_paged_kv_t) and of one step's rows
+// (fmoe_paged_batch_t), shared by the page operators (paged.cu) and attention.
+#pragma once
+#include "internal.h"
+#include "common.cuh"
+
+namespace fmoe {
+
+struct PagedDev {
+  uint8_t* pages;
+  int32_t *table, *lens, *refs, *refused;
+  int layers, Hkv, D, ps, log_ps, bits, num_pages, max_seqs, max_blocks;
+  int64_t block, page, layer;  // bytes: one head's K or V block, one page of one layer, one layer
+};
+struct BatchDev {
+  const int32_t *seqs, *q_start, *kv_len;
+  int n, max_new;
+  int64_t tokens;
+};
+
+// One head's K (which 0) or V (which 1) block of a page; 64-bit offsets: a pool
+// passes 4 GB long before its page ids pass 32 bits.
+__device__ __forceinline__ uint8_t* page_block(const PagedDev& c, int layer, int page, int h, int which) {
+  return c.pages + layer * c.layer + page * c.page + (2 * h + which) * c.block;
+}
+// Page of a block of table row `seq`; -1 where the table has none that exists.
+__device__ __forceinline__ int page_of(const PagedDev& c, int seq, int64_t blk) {
+  if (seq < 0 || seq >= c.max_seqs || blk < 0 || blk >= c.max_blocks) return -1;
+  const int p = __ldg(c.table + (int64_t)seq * c.max_blocks + blk);
+  return p < c.num_pages ? p : -1;
+}
+
+int paged_to_dev(const fmoe_paged_kv_t* c, PagedDev* d, bool need_pages);
+int batch_to_dev(const fmoe_paged_batch_t* b, BatchDev* d);
+
+}  // namespace fmoe

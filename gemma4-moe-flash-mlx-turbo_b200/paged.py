@@ -1,0 +1,300 @@
+"""Paged KV cache for many sequences (fmoe_paged_*; no counterpart in the
+reference, whose engine keeps one growing cache per sequence, src/cache.rs:161-310).
+
+    PagedKVCache    pages of bf16 or 4-bit rows that the sequences of a server take,
+                    share and give back: reserve, fork, free, trim, compact
+    PagedBatch      one step's rows: which sequences, how many new positions each
+    QKNormRope      norms and rotation of a layer's projections
+
+One step of a server:
+
+    batch = cache.reserve(seqs, new)                       room for the new positions
+    for layer ...:
+        q = cache.append_qkv(layer, q, k, v, batch, norm)  norms, rotation, rows -> pages
+        o = cache.attend(layer, q, batch, window, sinks)   every new row's attention
+
+Sequences are rows of the cache's block table (0 .. max_seqs - 1, the caller's to
+give out).  Ids and counts may be Python lists or int32 tensors on the device;
+with tensors no call waits for the GPU.  Calls run on the current stream, which
+orders them; scratch memory is kept for each stream.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _need_cuda, _ptr, _stream, check, lib
+
+
+class PagedKvC(ctypes.Structure):
+    _fields_ = [
+        ("layers", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("bits", ctypes.c_int32), ("num_pages", ctypes.c_int32),
+        ("max_seqs", ctypes.c_int32), ("max_blocks", ctypes.c_int32),
+        ("pages", ctypes.c_void_p), ("table", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+        ("refs", ctypes.c_void_p), ("refused", ctypes.c_void_p),
+    ]
+
+
+class PagedBatchC(ctypes.Structure):
+    _fields_ = [
+        ("n", ctypes.c_int32), ("max_new", ctypes.c_int32), ("tokens", ctypes.c_int64),
+        ("seqs", ctypes.c_void_p), ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+    ]
+
+
+class QKNormRopeC(ctypes.Structure):
+    _fields_ = [
+        ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float),
+        ("rope_theta", ctypes.c_float), ("rope_dims", ctypes.c_int32),
+    ]
+
+
+def _ids(x, device, what):
+    """A list, or an int32 tensor on the device, as the latter."""
+    if isinstance(x, torch.Tensor):
+        if x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous() or x.device != device:
+            raise ValueError(f"paged: {what} must be a contiguous int32 vector on {device}")
+        return x
+    x = [int(v) for v in x]
+    return torch.tensor(x, dtype=torch.int32).to(device)
+
+
+def _distinct(x, what):
+    if not isinstance(x, torch.Tensor) and len(set(x)) != len(x):
+        raise ValueError(f"paged: {what} {list(x)} name a sequence twice")
+
+
+class PagedBatch:
+    """The rows of one step.  seqs [n], q_start [n + 1] and kv_len [n] are int32
+    tensors on the device: sequence i's rows are q_start[i] .. q_start[i + 1] - 1
+    of the step's `tokens` rows, its positions kv_len[i] - (number of rows) ..
+    kv_len[i] - 1.  max_new bounds every sequence's rows."""
+
+    def __init__(self, seqs, q_start, kv_len, tokens: int, max_new: int):
+        _need_cuda(seqs, q_start, kv_len)
+        n = seqs.numel()
+        for t, size, what in ((seqs, n, "seqs"), (q_start, n + 1, "q_start"), (kv_len, n, "kv_len")):
+            if t.numel() != size or t.device != seqs.device:
+                raise ValueError(f"paged: {what} has {t.numel()} entries on {t.device}, {size} on {seqs.device} expected")
+            _ids(t, t.device, what)
+        if max_new < 0 or tokens < 0 or tokens > n * max_new:
+            raise ValueError(f"paged: {tokens} rows of {n} sequences with at most {max_new} each")
+        self.seqs, self.q_start, self.kv_len = seqs, q_start, kv_len
+        self.n, self.tokens, self.max_new = n, tokens, max_new
+        self.c = PagedBatchC(n, max_new, tokens, _ptr(seqs), _ptr(q_start), _ptr(kv_len))
+        self._ref = ctypes.byref(self.c)
+
+
+class QKNormRope:
+    """q_norm / k_norm bf16 [head_dim]; the first rope_dims dims turn in the pairs
+    (i, i + rope_dims / 2) at rope_theta^(-2i / rope_dims) per position."""
+
+    def __init__(self, q_norm, k_norm, rope_dims: int, rope_theta: float, eps: float = 1e-6):
+        _need_cuda(q_norm, k_norm)
+        if q_norm.shape != k_norm.shape or q_norm.dim() != 1:
+            raise ValueError(f"paged: q_norm {tuple(q_norm.shape)} and k_norm {tuple(k_norm.shape)} [head_dim] expected")
+        self.q_norm, self.k_norm = (w.to(torch.bfloat16).contiguous() for w in (q_norm, k_norm))
+        self.c = QKNormRopeC(_ptr(self.q_norm), _ptr(self.k_norm), eps, rope_theta, rope_dims)
+        self._ref = ctypes.byref(self.c)
+
+
+class PagedKVCache:
+    """layers x num_pages pages of page_size positions, and the block table of
+    max_seqs sequences of up to max_blocks pages.  bits 16: bf16 rows; 4: rows
+    quantised in groups of 64."""
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, num_pages: int, max_seqs: int, max_blocks: int,
+                 page_size: int = 32, bits: int = 16, device=None):
+        device = torch.device("cuda") if device is None else torch.device(device)
+        shape = PagedKvC(layers, kv_heads, head_dim, page_size, bits, num_pages, max_seqs, max_blocks)
+        nbytes = lib().fmoe_paged_bytes(ctypes.byref(shape))
+        if nbytes == 0:
+            check(lib().fmoe_paged_free(ctypes.byref(shape), None, 0, None))  # the shape's error
+        self._set(torch.empty(nbytes, dtype=torch.uint8, device=device),
+                  torch.full((max_seqs, max_blocks), -1, dtype=torch.int32, device=device),
+                  torch.zeros(max_seqs, dtype=torch.int32, device=device),
+                  torch.zeros(num_pages, dtype=torch.int32, device=device), shape)
+
+    @classmethod
+    def over(cls, pages, table, lens, refs, kv_heads: int, head_dim: int, page_size: int, bits: int = 16):
+        """A cache over memory that the caller has: pages [layers, num_pages, ...]
+        contiguous, table int32 [max_seqs, max_blocks], lens int32 [max_seqs], refs
+        int32 [num_pages]."""
+        _need_cuda(pages, table, lens, refs)
+        for t, what in ((table, "table"), (lens, "lens"), (refs, "refs")):
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.device != pages.device:
+                raise ValueError(f"paged: {what} must be contiguous int32 on {pages.device}")
+        if table.dim() != 2 or lens.numel() != table.shape[0] or not pages.is_contiguous() or pages.dim() < 2 or \
+                refs.numel() != pages.shape[1]:
+            raise ValueError(f"paged: pages {tuple(pages.shape)}, table {tuple(table.shape)}, lens {tuple(lens.shape)}, "
+                             f"refs {tuple(refs.shape)} do not belong together")
+        shape = PagedKvC(pages.shape[0], kv_heads, head_dim, page_size, bits, refs.numel(), *table.shape)
+        nbytes = lib().fmoe_paged_bytes(ctypes.byref(shape))
+        if nbytes == 0:
+            check(lib().fmoe_paged_free(ctypes.byref(shape), None, 0, None))
+        if pages.numel() * pages.element_size() != nbytes:
+            raise ValueError(f"paged: pages of {pages.numel() * pages.element_size()} bytes, {nbytes} expected")
+        self = object.__new__(cls)
+        self._set(pages, table, lens, refs, shape)
+        return self
+
+    def _set(self, pages, table, lens, refs, shape):
+        self.pages, self.table, self.lens, self.refs = pages, table, lens, refs
+        self.refused = torch.zeros(1, dtype=torch.int32, device=pages.device)
+        self.layers, self.kv_heads, self.head_dim = shape.layers, shape.kv_heads, shape.head_dim
+        self.page_size, self.bits, self.num_pages = shape.page_size, shape.bits, shape.num_pages
+        self.max_seqs, self.max_blocks = shape.max_seqs, shape.max_blocks
+        self.device = pages.device
+        shape.pages, shape.table, shape.lens = _ptr(pages), _ptr(table), _ptr(lens)
+        shape.refs, shape.refused = _ptr(refs), _ptr(self.refused)
+        self.c = shape
+        self._ref = ctypes.byref(self.c)
+        self._op_bytes = lib().fmoe_paged_workspace_bytes(self._ref)
+        self._scratch = {}
+
+    def _ws(self, kind, nbytes, stream):
+        """Scratch of one stream, grown when a call needs more; zeroed when allocated."""
+        buf = self._scratch.get((kind, stream))
+        if buf is None or buf.numel() < nbytes:
+            buf = self._scratch[kind, stream] = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
+        return buf
+
+    # -- pages ---------------------------------------------------------------
+    def reserve(self, seqs, new, tokens: int | None = None, max_new: int | None = None) -> PagedBatch:
+        """Room for new[i] more positions of sequence seqs[i]; returns the step's
+        batch.  With device tensors, tokens (rows of the step) and max_new have to be
+        given.  A sequence that there is no room for gets kv_len -1 in the batch (its
+        rows come back as zeros), keeps its length, and counts in `refused`."""
+        _distinct(seqs, "seqs")
+        if isinstance(new, torch.Tensor):
+            if tokens is None or max_new is None:
+                raise ValueError("paged: reserve with counts on the device needs tokens and max_new")
+            new = _ids(new, self.device, "new")
+            q_start = torch.zeros(new.numel() + 1, dtype=torch.int32, device=self.device)
+            torch.cumsum(new, 0, dtype=torch.int32, out=q_start[1:])
+        else:
+            new = [int(v) for v in new]
+            if any(v < 0 for v in new):
+                raise ValueError(f"paged: negative counts {new}")
+            ends = [0]
+            for v in new:
+                ends.append(ends[-1] + v)
+            tokens, max_new = ends[-1], max(new, default=0)
+            q_start, new = _ids(ends, self.device, "q_start"), _ids(new, self.device, "new")
+        seqs = _ids(seqs, self.device, "seqs")
+        if seqs.numel() != new.numel():
+            raise ValueError(f"paged: {seqs.numel()} sequences, {new.numel()} counts")
+        kv_len = torch.empty(seqs.numel(), dtype=torch.int32, device=self.device)
+        st = _stream()
+        ws = self._ws("op", self._op_bytes, st)
+        check(lib().fmoe_paged_reserve(self._ref, _ptr(seqs), _ptr(new), seqs.numel(), _ptr(kv_len), _ptr(ws),
+                                       ws.numel(), st))
+        return PagedBatch(seqs, q_start, kv_len, tokens, max_new)
+
+    def fork(self, parents, children) -> None:
+        """children[i] becomes a copy of parents[i]: full pages are shared, a last
+        page that is part full is copied.  No child may be a parent."""
+        _distinct(children, "children")
+        if not isinstance(parents, torch.Tensor) and not isinstance(children, torch.Tensor) and \
+                set(parents) & set(children):
+            raise ValueError(f"paged: {sorted(set(parents) & set(children))} are both parents and children")
+        a, b = _ids(parents, self.device, "parents"), _ids(children, self.device, "children")
+        if a.numel() != b.numel():
+            raise ValueError(f"paged: {a.numel()} parents, {b.numel()} children")
+        st = _stream()
+        ws = self._ws("op", self._op_bytes, st)
+        check(lib().fmoe_paged_fork(self._ref, _ptr(a), _ptr(b), a.numel(), _ptr(ws), ws.numel(), st))
+
+    def free(self, seqs) -> None:
+        """Gives back the sequences' pages."""
+        _distinct(seqs, "seqs")
+        s = _ids(seqs, self.device, "seqs")
+        check(lib().fmoe_paged_free(self._ref, _ptr(s), s.numel(), _stream()))
+
+    def trim(self, seqs, window: int, sinks: int = 0) -> None:
+        """Gives back the sequences' pages that no later position sees under the window."""
+        _distinct(seqs, "seqs")
+        s = _ids(seqs, self.device, "seqs")
+        check(lib().fmoe_paged_trim(self._ref, _ptr(s), s.numel(), window, sinks, _stream()))
+
+    def compact(self) -> torch.Tensor:
+        """Moves the live pages to the front of the pool; their number, int32 [1]."""
+        live = torch.empty(1, dtype=torch.int32, device=self.device)
+        st = _stream()
+        ws = self._ws("op", self._op_bytes, st)
+        check(lib().fmoe_paged_compact(self._ref, _ptr(live), _ptr(ws), ws.numel(), st))
+        return live
+
+    def copy_pages(self, src, dst) -> None:
+        """Page src[i] to page dst[i] in every layer."""
+        if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor) and \
+                (len(set(dst)) != len(dst) or set(src) & set(dst)):
+            raise ValueError("paged: copy_pages with a page twice in dst, or in both src and dst")
+        a, b = _ids(src, self.device, "src"), _ids(dst, self.device, "dst")
+        if a.numel() != b.numel():
+            raise ValueError(f"paged: {a.numel()} src, {b.numel()} dst")
+        check(lib().fmoe_paged_copy(self._ref, _ptr(a), _ptr(b), a.numel(), _stream()))
+
+    # -- a step's rows ---------------------------------------------------------
+    def _rows(self, x, heads, batch, what):
+        """A step's rows [tokens, heads, head_dim] in bf16 with whole rows together,
+        and how far apart they are."""
+        if not x.is_cuda:
+            raise ValueError("fmoe: tensors must live on a CUDA device")
+        D = self.head_dim
+        if x.dim() != 3 or x.shape[0] != batch.tokens or x.shape[2] != D or (heads and x.shape[1] != heads):
+            raise ValueError(f"paged: {what} {tuple(x.shape)}, [{batch.tokens}, {heads or 'heads'}, {D}] expected")
+        if x.dtype != torch.bfloat16:
+            x = x.to(torch.bfloat16)
+        if x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != D) or x.stride(0) % 8 or \
+                x.stride(0) < x.shape[1] * D or x.data_ptr() % 16:
+            x = x.contiguous()
+            if x.data_ptr() % 16:
+                x = x.clone()
+        return x, x.stride(0) if x.shape[0] > 1 else x.shape[1] * D
+
+    def append(self, layer: int, k, v, batch: PagedBatch) -> None:
+        """Stores k and v [tokens, kv_heads, head_dim] as they are."""
+        k, ks = self._rows(k, self.kv_heads, batch, "k")
+        v, vs = self._rows(v, self.kv_heads, batch, "v")
+        check(lib().fmoe_paged_append(self._ref, layer, _ptr(k), ks, _ptr(v), vs, batch._ref, _stream()))
+
+    def append_qkv(self, layer: int, q, k, v, batch: PagedBatch, norm: QKNormRope, out=None) -> torch.Tensor:
+        """Norms and turns the projections q [tokens, q_heads, head_dim], k and v
+        [tokens, kv_heads, head_dim] (v None: the raw keys), stores k and v and
+        returns q."""
+        q, qs = self._rows(q, 0, batch, "q")
+        k, ks = self._rows(k, self.kv_heads, batch, "k")
+        vs = 0
+        if v is not None:
+            v, vs = self._rows(v, self.kv_heads, batch, "v")
+        if norm.q_norm.numel() != self.head_dim:
+            raise ValueError(f"paged: norm weights of {norm.q_norm.numel()} values, head_dim {self.head_dim}")
+        out = self._out(out, q)
+        check(lib().fmoe_paged_append_qkv(self._ref, layer, _ptr(q), qs, q.shape[1], _ptr(k), ks, _ptr(v), vs,
+                                          batch._ref, norm._ref, _ptr(out), _stream()))
+        return out
+
+    def _out(self, out, q):
+        if out is None:
+            return torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        if out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != q.device:
+            raise ValueError(f"paged: out must be contiguous bf16 {tuple(q.shape)} on {q.device}")
+        return out
+
+    def attend(self, layer: int, q, batch: PagedBatch, window: int | None = None, sinks: int = 0, scale: float = 1.0,
+               out=None) -> torch.Tensor:
+        """Attention of q [tokens, q_heads, head_dim] over the layer's pages, the
+        batch's own rows among them: position p sees j <= p with j > p - window
+        (window None or 0: all) or j < sinks.  bf16 [tokens, q_heads, head_dim]."""
+        q, qs = self._rows(q, 0, batch, "q")
+        out = self._out(out, q)
+        heads = q.shape[1]
+        nbytes = lib().fmoe_paged_attend_workspace_bytes(self._ref, heads, batch.n, batch.tokens, batch.max_new)
+        st = _stream()
+        ws = self._ws("attend", nbytes, st)
+        check(lib().fmoe_paged_attend(self._ref, layer, _ptr(q), qs, heads, batch._ref, window or 0, sinks, scale,
+                                      _ptr(out), _ptr(ws), ws.numel(), st))
+        return out

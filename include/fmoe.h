@@ -307,6 +307,146 @@ int fmoe_attn_decode_sparse_v(const fmoe_kv_cache_t* cache, const void* q, int q
 int fmoe_turbo_round_trip(const void* x, int64_t rows, int head_dim, int bits, void* out,
                           void* stream);
 
+/* ---- paged KV cache ------------------------------------------------------ */
+
+/* A cache for many sequences that come, grow, share beginnings and go
+ * independently of one another (the reference keeps one growing cache per
+ * sequence, src/cache.rs:161-310; this has no counterpart there).  Rows live in
+ * pages of page_size positions, taken from one pool for all sequences; a block
+ * table maps block b of a sequence (positions b * page_size ...) to a page,
+ * the same one in each of the cache's layers.
+ *
+ * pages: [layers][num_pages][kv_heads][K, V][block].  bits 16: a block is bf16
+ * [page_size][head_dim].  bits 4: [page_size][head_dim / 8] 32-bit words of
+ * codes, then [page_size][head_dim / 64] pairs of bf16 (scale, bias); a value
+ * is scale * code + bias of its row's group of 64 (quantised as fmoe_quantize
+ * does).  The word of octet o (8 values) of group g is word
+ * o * (head_dim / 64) + g of the row, and value i of the octet is nibble
+ * (i >> 1) + 4 * (i & 1): a reader that owns an octet finds all groups' words
+ * side by side, and one mask takes two neighbouring values out of a word.
+ *
+ * The table and the counts live on the device, so that a captured decode loop
+ * can grow, fork and free; entries and ids that point outside the pool or the
+ * table are never followed. */
+typedef struct fmoe_paged_kv {
+  int32_t layers;
+  int32_t kv_heads;
+  int32_t head_dim;   /* 256 or 512 */
+  int32_t page_size;  /* positions per page: 16, 32, 64 or 128 */
+  int32_t bits;       /* 16 or 4 */
+  int32_t num_pages;
+  int32_t max_seqs;
+  int32_t max_blocks; /* entries of a sequence's table row */
+  void* pages;        /* fmoe_paged_bytes, 128-byte aligned */
+  int32_t* table;     /* [max_seqs][max_blocks], -1: no page */
+  int32_t* lens;      /* [max_seqs] positions held */
+  int32_t* refs;      /* [num_pages] table rows that hold the page; 0: free */
+  int32_t* refused;   /* [1] sequences that a reserve or fork could not serve */
+} fmoe_paged_kv_t;
+
+/* The rows of one step: n sequences, sequence i with the new positions
+ * kv_len[i] - new .. kv_len[i] - 1, new = q_start[i + 1] - q_start[i], whose
+ * rows are q_start[i] .. of the step's tensors.  seqs: their table rows.  All
+ * on the device; max_new bounds every sequence's new positions.  Rows at
+ * q_start[n] and after belong to no sequence and are not touched. */
+typedef struct fmoe_paged_batch {
+  int32_t n;
+  int32_t max_new;
+  int64_t tokens; /* rows of the step's tensors, >= q_start[n] */
+  const int32_t* seqs;
+  const int32_t* q_start; /* [n + 1], ascending from 0 */
+  const int32_t* kv_len;  /* [n] */
+} fmoe_paged_batch_t;
+
+/* Bytes of the pool that the shape asks for (0: unsupported shape), and of the
+ * workspace of reserve, fork and compact (no initialisation needed). */
+size_t fmoe_paged_bytes(const fmoe_paged_kv_t* cache);
+size_t fmoe_paged_workspace_bytes(const fmoe_paged_kv_t* cache);
+
+/* Room for counts[i] >= 0 more positions of sequence seqs[i] (distinct): takes
+ * the lowest free pages in the order of the sequences, adds counts to lens and
+ * writes the new lengths to kv_len.  A sequence that the pool or its table row
+ * has no room for, after those before it, stays as it is: its kv_len is -1,
+ * which the calls below take as a sequence without positions, and *refused
+ * grows by one. */
+int fmoe_paged_reserve(const fmoe_paged_kv_t* cache, const int32_t* seqs, const int32_t* counts, int n,
+                       int32_t* kv_len, void* workspace, size_t workspace_bytes, void* stream);
+
+/* children[i] becomes a copy of parents[i]: whole pages are shared, a last page
+ * that is only part full is copied in every layer to the lowest free page (in
+ * the order of the pairs), so that both can grow.  What a child held is freed
+ * first.  No child may be a parent or a child twice; such pairs, ids outside
+ * the table and pairs without a free page count in *refused (the last leave
+ * the child empty, the others leave it as it is). */
+int fmoe_paged_fork(const fmoe_paged_kv_t* cache, const int32_t* parents, const int32_t* children, int n,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Lets go of all pages of n distinct sequences. */
+int fmoe_paged_free(const fmoe_paged_kv_t* cache, const int32_t* seqs, int n, void* stream);
+
+/* Lets go of the pages of n distinct sequences that no later position sees
+ * under a window (> 0) with `sinks` first positions that stay visible. */
+int fmoe_paged_trim(const fmoe_paged_kv_t* cache, const int32_t* seqs, int n, int window, int sinks, void* stream);
+
+/* Brings the live pages to the front of the pool: the k-th live page at or past
+ * the number of live pages moves to the k-th free page before it, in every
+ * layer, and the table follows.  *live (device) receives that number: the pages
+ * from it on are free. */
+int fmoe_paged_compact(const fmoe_paged_kv_t* cache, int32_t* live, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* Copies page src[i] to dst[i] in every layer (device ids; no dst twice, and no
+ * page both a src and a dst). */
+int fmoe_paged_copy(const fmoe_paged_kv_t* cache, const int32_t* src, const int32_t* dst, int n, void* stream);
+
+/* Stores the batch's new rows of one layer as they are (bits 4: quantised):
+ * k, v bf16 [tokens][kv_heads][head_dim], rows k_stride / v_stride values
+ * apart (multiples of 8; 16-byte aligned).  Positions without a page are
+ * dropped. */
+int fmoe_paged_append(const fmoe_paged_kv_t* cache, int layer, const void* k, int64_t k_stride, const void* v,
+                      int64_t v_stride, const fmoe_paged_batch_t* batch, void* stream);
+
+/* Norms and rotation of the heads of one layer's projections,
+ * Gemma4Attention::forward (src/model/gemma4_attention.rs:46-84): q and k rows
+ * are RMS-normed and multiplied by their weights, v rows RMS-normed without
+ * one; q and k turn in the pairs (i, i + rope_dims / 2) of their first
+ * rope_dims values by position * rope_theta^(-2i / rope_dims). */
+typedef struct fmoe_qk_norm_rope {
+  const void* q_norm; /* bf16 [head_dim] */
+  const void* k_norm;
+  float eps;
+  float rope_theta;
+  int32_t rope_dims; /* 0..head_dim, a multiple of head_dim / 16 */
+} fmoe_qk_norm_rope_t;
+
+/* The norms and the rotation of a batch's new rows in one pass that also
+ * stores k and v in the pages: q [tokens][q_heads][head_dim], k and v
+ * [tokens][kv_heads][head_dim], bf16, rows *_stride values apart (multiples of
+ * 8; 16-byte aligned); v NULL: the values are the raw keys.  q_out bf16
+ * [tokens][q_heads][head_dim].  32-bit arithmetic, one rounding at the store
+ * (bits 4: quantised from the 32-bit values); angles reduced in 64 bits. */
+int fmoe_paged_append_qkv(const fmoe_paged_kv_t* cache, int layer, const void* q, int64_t q_stride, int q_heads,
+                          const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                          const fmoe_paged_batch_t* batch, const fmoe_qk_norm_rope_t* norm, void* q_out, void* stream);
+
+/* Attention of the batch's new rows over one layer's pages (the new rows
+ * stored before).  q [tokens][q_heads][head_dim] bf16, rows q_stride values
+ * apart (a multiple of 8; 16-byte aligned); query head h reads kv head
+ * h / (q_heads / kv_heads), 1..8 query heads to a kv head.  The query at
+ * position p sees position j <= p if window == 0, j > p - window or j < sinks,
+ * and if j's block has a page; rows that see nothing are zero.
+ *   out[t, h] = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max),  s_j = scale * q[t, h] . k_j
+ * Rows of positions that no query of the sequence sees are not used, whatever
+ * they hold; among those that one query sees and another does not, values must
+ * be finite.  The workspace must be zero-filled before its first use; every
+ * call leaves its counters at zero.  Calls sharing one must not overlap on the
+ * GPU. */
+size_t fmoe_paged_attend_workspace_bytes(const fmoe_paged_kv_t* cache, int q_heads, int32_t n, int64_t tokens,
+                                         int32_t max_new);
+int fmoe_paged_attend(const fmoe_paged_kv_t* cache, int layer, const void* q, int64_t q_stride, int q_heads,
+                      const fmoe_paged_batch_t* batch, int window, int sinks, float scale, void* out,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- decoder layer + lm_head (decode step) ----------------------------- */
 
 /* One Gemma-4 decoder layer, DecoderLayer::forward_gemma4 (src/model/mod.rs:
