@@ -1,0 +1,49 @@
+// Shared by the kernels of attention over pages (pattn.cu, pattn_tc.cu).
+#pragma once
+#include "paged.cuh"
+#include "stage.cuh"
+
+namespace fmoe {
+namespace pa {
+
+struct AttnArgs {
+  const bf16* q;  // [tokens][Hq][D], rows qs values apart
+  bf16* out;      // [tokens][Hq][D]
+  int64_t qs;
+  int Hq, share, layer, window, sinks;  // share: query heads of a kv head
+  float sl;                             // scale * log2(e): weights are powers of two
+};
+
+// Sequences of at most this many (row, head of the kv head's group) pairs run
+// on the split kernel, which holds them as the 8 columns of its products.
+constexpr int kFewRows = 8;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What the rows at positions p0 .. p1 of one sequence see, in tiles of T
+// positions: tiles [0, ns) hold first positions that stay visible, then come
+// the tiles from `low_tile`; positions in [low, hi) or below `sinks` are seen by
+// some row.
+struct Span {
+  int low, hi, ns, low_tile, tiles;
+};
+template <int T>
+__host__ __device__ __forceinline__ Span span_of(int p0, int p1, int window, int sinks, int capacity) {
+  Span s;
+  s.hi = p1 < 0 ? 0 : p1 < capacity ? p1 + 1 : capacity;  // table rows hold `capacity` positions
+  s.low = window && p0 >= window ? p0 - window + 1 : 0;
+  if (s.low > s.hi) s.low = s.hi;
+  s.low_tile = s.low / T;
+  const int first = window ? (sinks < s.hi ? sinks : s.hi) : 0;
+  s.ns = (first + T - 1) / T;
+  if (s.ns > s.low_tile) s.ns = s.low_tile;
+  s.tiles = s.ns + (s.hi + T - 1) / T - s.low_tile;
+  return s;
+}
+
+}  // namespace pa
+}  // namespace fmoe
