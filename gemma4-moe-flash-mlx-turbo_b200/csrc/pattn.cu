@@ -22,14 +22,14 @@ namespace pa {
 //
 // The pages' bytes are what a decode costs, so the work is cut by them: all
 // (sequence, kv head) items' keys form one line of granules of 16 positions (a
-// granule never leaves its page), and every CTA takes the same length of it,
-// whatever the sequences' lengths are.  A warp owns every 8th granule of its
-// CTA's part and has its own ring of TMA copies, running maximum, sum and
-// output, so that nothing in the loop waits for another warp and the copies run
-// on across the ends of items.  At the end of an item its warps' results are
-// joined in shared memory; an item that lies in several CTAs goes to scratch
-// and paged_attn_join_kernel joins its parts in the order of the keys: no
-// result depends on who arrives first.
+// granule never leaves its page), and every CTA, and in it every warp, takes the
+// same length of it, whatever the sequences' lengths are.  A warp has its own
+// ring of TMA copies, running maximum, sum and output, so that nothing in the
+// loop waits for another warp and the copies run on across the ends of items.
+// An item inside one warp's part is written by it; parts of an item in several
+// warps are joined at the end of the CTA, parts in several CTAs by
+// paged_attn_join_kernel, in the order of the keys: no result depends on who
+// arrives first.
 //
 // One granule, with the 8 columns being the item's (row, head) pairs:
 //   S^T [16 keys x 8]   = K  [16 x D] Q^T    mma m16n8k16, A = K  (ldmatrix)
@@ -48,43 +48,53 @@ namespace pa {
 template <int D_, int BITS_>
 struct Few {
   static constexpr int D = D_, BITS = BITS_, NG = D / 64;
-  static constexpr int NW = 8, NT = 32 * NW;
-  // A ring piece: 16 keys of K or V, bf16 in steps of 256 dims (8 KB), 4-bit
-  // whole rows and their (scale, bias) pairs.  Its boxes are 16 rows of 128
-  // bytes, swizzled.
-  static constexpr int H = BITS == 16 ? D / 256 : 1;  // pieces of a granule's K
-  static constexpr int BOXES = BITS == 16 ? 4 : D / 256, CODES = 2048 * BOXES;
-  static constexpr int PAIRS = BITS == 4 ? D : 0;
-  static constexpr int PIECE = BITS == 16 ? CODES : (CODES + PAIRS + 1023) / 1024 * 1024;
-  static constexpr int NP = BITS == 16 ? 3 : D == 256 ? 7 : 4;  // pieces in a warp's ring
-  static constexpr int OS = D + 4;                              // row stride of a joined output, floats
-  static constexpr int MW = D == 256 ? 2 : 1;                   // warps that hand over their output at a time
-  static constexpr int MAXSEG = 32;
-  static constexpr int OFF_O = NW * NP * PIECE, OFF_Q = OFF_O + MW * 8 * OS * 4, OFF_ML = OFF_Q + 16 * D;
-  static constexpr int OFF_SEG = OFF_ML + NW * 16 * 4, OFF_BAR = OFF_SEG + MAXSEG * 64;
+  // 4-bit granules cost more instructions than copies take: twelve warps hide
+  // more of their latency than eight where the registers allow it.
+  static constexpr int NW = D == 256 && BITS == 4 ? 12 : 8, NT = 32 * NW;
+  // A ring piece is one copy group: bf16 16 keys x 256 dims of K or V (8 KB);
+  // 4-bit a whole granule, K's and V's codes and (scale, bias) pairs.  Its boxes
+  // are 16 rows of 128 bytes, swizzled.
+  static constexpr int H = D / 256;                 // bf16: pieces of a granule's K
+  static constexpr int PER = BITS == 16 ? 2 * H : 1;  // pieces of a granule
+  static constexpr int CODES = BITS == 16 ? 8192 : 8 * D, PAIRS = BITS == 4 ? D : 0;
+  static constexpr int PIECE = BITS == 16 ? CODES : (2 * (CODES + PAIRS) + 1023) / 1024 * 1024;
+  static constexpr int NP = BITS == 16 || D == 256 ? 3 : 2;  // pieces in a warp's ring
+  static constexpr bool QREG = BITS == 16 || D == 256;       // q's fragments in registers, else in shared memory
+  static constexpr int MAXSEG = 64;
+  static constexpr int OFF_Q = NW * NP * PIECE, OFF_SEG = OFF_Q + (QREG ? 0 : NW * 16 * D);
+  static constexpr int OFF_PART = OFF_SEG + MAXSEG * 64, OFF_ML = OFF_PART + 2 * NW * 32;
+  static constexpr int OFF_BAR = OFF_ML + 2 * NW * 64;
   static constexpr int SMEM = OFF_BAR + NW * NP * 8 + 1024;  // the swizzle wants 1024-byte boxes
-  static constexpr int VPT = 8 * D / NT;                     // joined values of a thread
-  static_assert(SMEM <= 227 * 1024 - 256, "shared memory");
+  static constexpr int FRAGS = 2 * D;                        // float4s of an output: D / 16 tiles x 32 lanes
+  static_assert(SMEM <= 227 * 1024 - 2048, "shared memory");
+  static_assert(NP * PIECE >= 32 * D, "a part fits a ring");
 };
 
-// One item's part that lies in this CTA.
+// One item that lies in this CTA, or in part.
 struct Seg {
-  int seq, h, row0, rows;      // table row, kv head, first row of the step, its (row, head) pairs
-  int p0, i0, i1, first_slot;  // position of the first row; this part's granules; where the item's first part goes
-  int low, hi, ns, low_tile;   // its Span
-  int whole, cf, cl, slot;     // 1: no other part; CTAs that hold it; where this part goes
+  int seq, h, row0, rows;     // table row, kv head, first row of the step, its (row, head) pairs
+  int p0, s0, ng, first_slot; // position of the first row; granules: where it begins in the CTA's part, how many;
+                              // where its first part goes
+  int low, hi, ns, low_tile;  // its Span
+  int item, cf, cl, slot;     // its number on the line; CTAs that hold it; where this CTA's part goes
 };
-static_assert(sizeof(Seg) == 64, "segment list");
-
+// What a warp's part of an item leaves, for the CTA to join.
+struct Part {
+  int item, row0, rows, h, cf, cl, slot, in_ring;
+};
 // An item that ends in a CTA and began in an earlier one, for the join.
 struct Split {
   int row0, rows, h, cf, first_slot, pad[3];
 };
+static_assert(sizeof(Seg) == 64 && sizeof(Part) == 32 && sizeof(Split) == 32, "lists");
+
+// An output in scratch is [D / 16][32 lanes][4]: the fragments as they are.
 struct FewWs {
   int* status;
   Split* split;  // [grid]; rows 0: none
-  float* o;      // [2 * grid][8][D]
+  float* o;      // [2 * grid][8 * D] parts of CTAs
   float2* ml;    // [2 * grid][8]
+  float* wo;     // [grid][NW][8 * D] parts of warps
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -144,8 +154,28 @@ __device__ __forceinline__ void reset(Acc<C>& x) {
 
 // Adds piece hf of K to the scores of one granule.
 template <class C>
-__device__ __forceinline__ void scores(uint32_t kp, uint32_t qs, int hf, const float (&xs)[C::NG][2], int lane,
-                                       float (&s)[4]) {
+struct Query {
+  uint4 f[C::QREG ? C::D / 32 : 1];  // B fragments, two k steps to an entry
+  uint32_t at;                       // or where they are in shared memory
+  float sum[C::BITS == 4 ? C::NG : 1][2];  // 4-bit: sums of q over the groups, columns 2t and 2t + 1
+  __device__ __forceinline__ uint4 frag(int i, int lane) const {
+    if constexpr (C::QREG)
+      return f[i];
+    else
+      return lds128(at + (i * 32 + lane) * 16);
+  }
+};
+
+// acc.x += a * b.x, acc.y += a * b.y as one packed operation
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float bx, float by) {
+  asm("{\n .reg .b64 p, q, r;\n mov.b64 p, {%2, %2};\n mov.b64 q, {%3, %4};\n mov.b64 r, {%0, %1};\n"
+      " fma.rn.f32x2 r, p, q, r;\n mov.b64 {%0, %1}, r;\n}\n"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(bx), "f"(by));
+}
+
+template <class C>
+__device__ __forceinline__ void scores(uint32_t kp, const Query<C>& q, int hf, int lane, float (&s)[4]) {
   const int g = lane >> 2, t = lane & 3;
   if constexpr (C::BITS == 16) {
     float acc[4][4];
@@ -154,11 +184,11 @@ __device__ __forceinline__ void scores(uint32_t kp, uint32_t qs, int hf, const f
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
     const int r = lane & 15;
-    const uint32_t q = qs + (hf * 256 + lane) * 16, sw = (r & 7) << 4;
+    const uint32_t sw = (r & 7) << 4;
     kp += r * 128;
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) {  // 32 dims
-      const uint4 b = lds128(q + kk * 512);
+      const uint4 b = q.frag(8 * hf + kk, lane);
       uint32_t a0[4], a1[4];
       ldsm4(kp + (kk >> 1) * 2048 + ((((4 * kk) & 7) * 16 + (lane & 16)) ^ sw), a0);
       ldsm4(kp + (kk >> 1) * 2048 + ((((4 * kk + 2) & 7) * 16 + (lane & 16)) ^ sw), a1);
@@ -181,7 +211,7 @@ __device__ __forceinline__ void scores(uint32_t kp, uint32_t qs, int hf, const f
           const uint4 v = lds128(kp + (ch >> 3) * 2048 + r * 128 + (((ch ^ r) & 7) << 4));
           w[i][o][0] = v.x, w[i][o][1] = v.y, w[i][o][2] = v.z, w[i][o][3] = v.w;
         }
-        const uint4 p = lds128(kp + C::CODES + r * (C::D / 16) + q4 * 16);
+        const uint4 p = lds128(kp + 2 * C::CODES + r * (C::D / 16) + q4 * 16);
         pr[i][0] = p.x, pr[i][1] = p.y, pr[i][2] = p.z, pr[i][3] = p.w;
       }
 #pragma unroll
@@ -190,7 +220,7 @@ __device__ __forceinline__ void scores(uint32_t kp, uint32_t qs, int hf, const f
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k2 = 0; k2 < 2; ++k2) {
-          const uint4 b = lds128(qs + ((gr * 2 + k2) * 32 + lane) * 16);
+          const uint4 b = q.frag(gr * 2 + k2, lane);
           mma16816(acc, nib_pair(w[0][0][e], 8 * k2), nib_pair(w[1][0][e], 8 * k2), nib_pair(w[0][1][e], 8 * k2),
                    nib_pair(w[1][1][e], 8 * k2), b.x, b.y);
           mma16816(acc, nib_pair(w[0][0][e], 8 * k2 + 4), nib_pair(w[1][0][e], 8 * k2 + 4),
@@ -199,8 +229,8 @@ __device__ __forceinline__ void scores(uint32_t kp, uint32_t qs, int hf, const f
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float sc = bf16lo(pr[i][e]), bi = fmaf(-128.f, sc, bf16hi(pr[i][e]));
-          s[2 * i] = fmaf(sc, acc[2 * i], fmaf(bi, xs[gr][0], s[2 * i]));
-          s[2 * i + 1] = fmaf(sc, acc[2 * i + 1], fmaf(bi, xs[gr][1], s[2 * i + 1]));
+          fma2(s[2 * i], s[2 * i + 1], bi, q.sum[gr][0], q.sum[gr][1]);
+          fma2(s[2 * i], s[2 * i + 1], sc, acc[2 * i], acc[2 * i + 1]);
         }
       }
     }
@@ -210,8 +240,8 @@ __device__ __forceinline__ void scores(uint32_t kp, uint32_t qs, int hf, const f
 // Piece hf of O^T += V^T P^T; p: the weights of rows g, g + 8 of the score
 // product and columns 2t, 2t + 1 (bf16: their transposed fragments in b0, b1).
 template <class C>
-__device__ __forceinline__ void add_values(uint32_t vp, int hf, const float (&p)[4], uint32_t b0, uint32_t b1, int lane,
-                                           Acc<C>& x) {
+__device__ __forceinline__ void add_values(uint32_t vp, uint32_t pairs, int hf, const float (&p)[4], uint32_t b0,
+                                           uint32_t b1, int lane, Acc<C>& x) {
   const int g = lane >> 2, t = lane & 3;
   if constexpr (C::BITS == 16) {
     const int r = (lane & 7) + ((lane >> 4) << 3);
@@ -236,7 +266,7 @@ __device__ __forceinline__ void add_values(uint32_t vp, int hf, const float (&p)
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint4 v = lds128(vp + C::CODES + (k0 + 8 * i) * (C::D / 16) + q4 * 16);
+        const uint4 v = lds128(pairs + (k0 + 8 * i) * (C::D / 16) + q4 * 16);
         pr[i][0] = v.x, pr[i][1] = v.y, pr[i][2] = v.z, pr[i][3] = v.w;
       }
 #pragma unroll
@@ -246,8 +276,10 @@ __device__ __forceinline__ void add_values(uint32_t vp, int hf, const float (&p)
         const uint32_t ps0 = pack_bf16x2(p[0] * s0, p[1] * s0), ps1 = pack_bf16x2(p[2] * s1, p[3] * s1);
         // v = s (c - 8) + (b + 8 s): only the first part carries the rounding of P s
         const float z0 = fmaf(8.f, s0, bf16hi(pr[0][e])), z1 = fmaf(8.f, s1, bf16hi(pr[1][e]));
-        x.corr[gr][0] = fmaf(-136.f, bf16lo(ps0) + bf16lo(ps1), fmaf(p[0], z0, fmaf(p[2], z1, x.corr[gr][0])));
-        x.corr[gr][1] = fmaf(-136.f, bf16hi(ps0) + bf16hi(ps1), fmaf(p[1], z0, fmaf(p[3], z1, x.corr[gr][1])));
+        fma2(x.corr[gr][0], x.corr[gr][1], z0, p[0], p[1]);
+        fma2(x.corr[gr][0], x.corr[gr][1], z1, p[2], p[3]);
+        fma2(x.corr[gr][0], x.corr[gr][1], -136.f, bf16lo(ps0), bf16hi(ps0));
+        fma2(x.corr[gr][0], x.corr[gr][1], -136.f, bf16lo(ps1), bf16hi(ps1));
         const uint32_t c0 = transpose8x8(ps0), c1 = transpose8x8(ps1);
         // the pair (key of slot 2t, of 2t + 1) of one dim in one register: even dims
         // of the octet are the low halves' nibbles, odd dims the high halves'
@@ -262,10 +294,33 @@ __device__ __forceinline__ void add_values(uint32_t vp, int hf, const float (&p)
   }
 }
 
-// Dim of element e of output tile mt in lane group g.
+// Rows of the step that the item's columns are, for the stores.
+struct Rows {
+  bf16* out;
+  int row0, rows, head0, share, Hq;
+  __device__ __forceinline__ bf16* row(int col, int D) const {
+    return out + ((int64_t)(row0 + col / share) * Hq + head0 + col % share) * D;
+  }
+};
+
+// Output tile mt, divided by the columns' sums, as this warp's lanes hold it.
+// bf16 pages: element e of lane (g, t) is dim 16 mt + g + 8 (e / 2); 4-bit:
+// 64 (mt / 4) + 8 g + 2 (mt % 4) + e / 2; column 2t + e % 2.
 template <class C>
-__device__ __forceinline__ int dim_of(int mt, int e, int g) {
-  return C::BITS == 16 ? 16 * mt + g + 8 * (e >> 1) : 64 * (mt >> 2) + 8 * g + 2 * (mt & 3) + (e >> 1);
+__device__ __forceinline__ void store_tile(const Rows& r, int mt, float4 v, float i0, float i1, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  if constexpr (C::BITS == 16) {
+    const uint32_t lo = transpose8x8(pack_bf16x2(v.x * i0, v.y * i1)), hi = transpose8x8(pack_bf16x2(v.z * i0, v.w * i1));
+    if (g < r.rows) {
+      uint32_t* o = reinterpret_cast<uint32_t*>(r.row(g, C::D) + 16 * mt + 2 * t);
+      o[0] = lo;
+      o[4] = hi;
+    }
+  } else {
+    const int d = 64 * (mt >> 2) + 8 * g + 2 * (mt & 3);
+    if (2 * t < r.rows) *reinterpret_cast<uint32_t*>(r.row(2 * t, C::D) + d) = pack_bf16x2(v.x * i0, v.z * i0);
+    if (2 * t + 1 < r.rows) *reinterpret_cast<uint32_t*>(r.row(2 * t + 1, C::D) + d) = pack_bf16x2(v.y * i1, v.w * i1);
+  }
 }
 
 template <class C>
@@ -276,14 +331,15 @@ __global__ void __launch_bounds__(C::NT, 1)
   extern __shared__ uint8_t sm_raw[];
   __shared__ int2 scan_sh[NW];
   __shared__ int seg_n, failed_sh;
+  __shared__ int tail_sh[2 * NW];
+  __shared__ float2 share_sh[2 * NW][8];  // a part's weight in its item's column, and 1 / the column's sum
   __shared__ int64_t item_sh;
   uint8_t* sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* ring = sm + warp * (NP * C::PIECE);
-  float* obuf = reinterpret_cast<float*>(sm + C::OFF_O);
-  uint32_t* qs = reinterpret_cast<uint32_t*>(sm + C::OFF_Q);
-  float2* ml = reinterpret_cast<float2*>(sm + C::OFF_ML);  // [NW][8]
   Seg* segs = reinterpret_cast<Seg*>(sm + C::OFF_SEG);
+  Part* parts = reinterpret_cast<Part*>(sm + C::OFF_PART);  // [NW][2]
+  float2* ml = reinterpret_cast<float2*>(sm + C::OFF_ML);   // [NW][2][8] (maximum, sum)
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR) + warp * NP;
   volatile int* failed = &failed_sh;
   const int capacity = c.max_blocks << c.log_ps;
@@ -292,6 +348,7 @@ __global__ void __launch_bounds__(C::NT, 1)
   if (lane < NP) mbar_init(&full[lane], 1);
   mbar_fence_init();
   if (tid == 0) failed_sh = 0;
+  if (lane < 2) parts[2 * warp + lane].item = -1;
 
   // What sequence k0 + tid has on the line, and the sums over the chunk's sequences.
   struct Mine {
@@ -339,7 +396,7 @@ __global__ void __launch_bounds__(C::NT, 1)
     }
     return m;
   };
-  Mine m0 = survey(0);
+  const Mine m0 = survey(0);
   auto chunk = [&](int k0) { return k0 == 0 ? m0 : survey(k0); };
 
   // the line of all granules (every kv head has the same), and this CTA's part of it
@@ -352,12 +409,18 @@ __global__ void __launch_bounds__(C::NT, 1)
     if (tid == 0) ws.split[blockIdx.x].rows = 0;
     return;
   }
+  // this warp's part of it, in granules from u0
+  const int w0 = (int)((u1 - u0) * warp / NW), w1 = (int)((u1 - u0) * (warp + 1) / NW);
 
-  int issued = 0, used = 0;  // pieces of this warp, over all rounds
-  for (int done = 0;;) {     // the segments of this part, MAXSEG at a time
+  int issued = 0, used = 0;  // pieces of this warp
+  uint32_t valid = 0;        // whether the granules on their way have a page, by their number modulo 32
+  int gi = 0, gu = 0;        // granules issued, used
+  int left = 0;              // parts of items that this warp has left
+  float* wo = ws.wo + ((int64_t)blockIdx.x * NW + warp) * 8 * D;
+  for (int done = 0;;) {     // the items of the CTA's part, MAXSEG at a time
     __syncthreads();
     if (tid == 0) seg_n = 0;
-    if (done == 0) {  // the item that this part begins in, as its number on the line
+    if (done == 0) {  // the item that the part begins in, as its number on the line
       int64_t base = 0, items = 0;
       for (int k0 = 0; k0 < b.n; k0 += NT) {
         const Mine m = chunk(k0);
@@ -371,7 +434,7 @@ __global__ void __launch_bounds__(C::NT, 1)
     __syncthreads();
     const int64_t item0 = item_sh + done;
     int64_t base = 0, items = 0;
-    for (int k0 = 0; k0 < b.n; k0 += NT) {  // each thread lists the segments of its sequence
+    for (int k0 = 0; k0 < b.n; k0 += NT) {  // each thread lists the items of its sequence
       const Mine m = chunk(k0);
       const int64_t U = base + (int64_t)m.at_u * c.Hkv, rel = (items + m.at_i) * c.Hkv - item0;
       if (m.ng > 0 && U < u1 && U + (int64_t)m.ng * c.Hkv > u0) {
@@ -384,15 +447,15 @@ __global__ void __launch_bounds__(C::NT, 1)
           s.row0 = m.first;
           s.rows = m.count * a.share;
           s.p0 = m.p0;
-          s.i0 = (int)(max(u0, s0) - s0);
-          s.i1 = (int)(min(u1, s0 + m.ng) - s0);
+          s.s0 = (int)(s0 - u0);
+          s.ng = m.ng;
           s.low = m.sp.low;
           s.hi = m.sp.hi;
           s.ns = m.sp.ns;
           s.low_tile = m.sp.low_tile;
-          s.cf = (int)(s0 / part);
-          s.cl = (int)((s0 + m.ng - 1) / part);
-          s.whole = s.cf == s.cl;
+          s.item = (int)(item0 + at);
+          s.cf = s0 >= u0 ? blockIdx.x : (int)(s0 / part);
+          s.cl = s0 + m.ng <= u1 ? blockIdx.x : (int)((s0 + m.ng - 1) / part);
           s.slot = 2 * blockIdx.x + (s0 > u0);
           s.first_slot = 2 * s.cf + (s0 > s.cf * part);
           segs[at] = s;
@@ -406,120 +469,156 @@ __global__ void __launch_bounds__(C::NT, 1)
     const int n_seg = seg_n;
     if (done == 0 && tid == 0) {  // only the part's first item can have begun before it
       const Seg& s = segs[0];
-      const bool ends = !s.whole && s.cf < (int)blockIdx.x && s.cl == (int)blockIdx.x;
       Split* r = ws.split + blockIdx.x;
       r->row0 = s.row0;
-      r->rows = ends ? s.rows : 0;
+      r->rows = s.cf < (int)blockIdx.x && s.cl == (int)blockIdx.x ? s.rows : 0;
       r->h = s.h;
       r->cf = s.cf;
       r->first_slot = s.first_slot;
     }
     if (n_seg == 0) break;
 
-    // -- this warp's copies: granules i0 + warp, + NW, ... of each segment, pieces of K then of V
-    int ls = 0, li = segs[0].i0 + warp, lp = 0, entry = -1, entry0 = 0, entry_s = -1;
-    auto settle = [&]() {  // on to the warp's next granule that exists
-      while (ls < n_seg && li >= segs[ls].i1)
-        if (++ls < n_seg) li = segs[ls].i0 + warp;
+    // -- this warp's copies: its granules in order, each one's pieces of K, then of V
+    int ls = 0, li = 0, lend = 0, lp = 0, entry = -1, entry0 = 0, page = -1;
+    auto enter = [&]() {  // the next item at or after ls with granules of this warp
+      for (; ls < n_seg; ++ls) {
+        const int s0 = segs[ls].s0;
+        li = max(w0 - s0, 0);
+        lend = min(w1 - s0, segs[ls].ng);
+        if (li < lend) break;
+      }
+      entry0 = -32;
     };
     auto issue = [&]() {
       if (ls >= n_seg || __any_sync(0xffffffffu, *failed)) return;
       const Seg& s = segs[ls];
-      const int k = (li - s.i0) / NW;
-      if (entry_s != ls || k >= entry0 + 32) {  // lanes hold the pages of the warp's next 32 granules
-        entry_s = ls;
-        entry0 = k;
-        const int j = li + lane * NW, tile = j < s.ns ? j : s.low_tile + j - s.ns;
-        entry = j < s.i1 ? page_of(c, s.seq, (16 * (int64_t)tile) >> c.log_ps) : -1;
-      }
-      const int page = __shfl_sync(0xffffffffu, entry, k - entry0);
       const int tile = li < s.ns ? li : s.low_tile + li - s.ns, slot = (16 * tile) & (c.ps - 1);
-      const int stage = issued % NP, which = lp >= H;
+      if (lp == 0) {
+        if (entry0 < 0 || li >= entry0 + 32) {  // lanes hold the pages of the next 32 granules
+          entry0 = li;
+          const int j = li + lane, tj = j < s.ns ? j : s.low_tile + j - s.ns;
+          entry = j < lend ? page_of(c, s.seq, (16 * (int64_t)tj) >> c.log_ps) : -1;
+        }
+        page = __shfl_sync(0xffffffffu, entry, li - entry0);
+        valid = (valid & ~(1u << (gi & 31))) | ((uint32_t)(page >= 0) << (gi & 31));
+        ++gi;
+      }
+      const int stage = issued % NP;
       uint8_t* dst = ring + stage * C::PIECE;
-      if (lane == 0) mbar_arrive_expect_tx(&full[stage], page >= 0 ? C::CODES + C::PAIRS : 0);
+      if (lane == 0)
+        mbar_arrive_expect_tx(&full[stage], page < 0 ? 0 : C::BITS == 16 ? C::CODES : 2 * (C::CODES + C::PAIRS));
       __syncwarp();
       if (page >= 0) {
-        const int blk = (page * c.Hkv + s.h) * 2 + which;
         if constexpr (C::BITS == 16) {
-          if (lane < 4) tc::tma2d(dst + lane * 2048, &map, (lp - which * H) * 256 + lane * 64, blk * c.ps + slot, &full[stage]);
-        } else {
-          if (lane < C::BOXES) tc::tma3d(dst + lane * 2048, &map, lane * 128, slot, blk, &full[stage]);
-          if (lane == C::BOXES)
-            bulk_g2s(dst + C::CODES, page_block(c, a.layer, page, s.h, which) + c.ps * (D / 2) + slot * (D / 16), C::PAIRS,
-                     &full[stage]);
+          const int which = lp >= H;
+          if (lane < 4)
+            tc::tma2d(dst + lane * 2048, &map, (lp - which * H) * 256 + lane * 64,
+                      ((page * c.Hkv + s.h) * 2 + which) * c.ps + slot, &full[stage]);
+        } else {  // K's boxes, V's boxes, their pairs
+          const int which = lane & 1, box = lane >> 1;
+          if (box < H)
+            tc::tma3d(dst + which * C::CODES + box * 2048, &map, box * 128, slot, (page * c.Hkv + s.h) * 2 + which, &full[stage]);
+          else if (box == H)
+            bulk_g2s(dst + 2 * C::CODES + which * C::PAIRS,
+                     page_block(c, a.layer, page, s.h, which) + c.ps * (D / 2) + slot * (D / 16), C::PAIRS, &full[stage]);
         }
       }
       ++issued;
-      if (++lp == 2 * H) {
+      if (++lp == C::PER) {
         lp = 0;
-        li += NW;
-        settle();
+        if (++li >= lend) {
+          ++ls;
+          enter();
+        }
       }
     };
-    settle();
+    enter();
 #pragma unroll 1
     for (int i = 0; i < NP; ++i) issue();
 
 #pragma unroll 1
     for (int si = 0; si < n_seg; ++si) {
-      const Seg s = segs[si];
-      // the item's 8 columns of q as B fragments, two k steps to a 16-byte read
+      const Seg& s = segs[si];
+      const int i0 = max(w0 - s.s0, 0), i1 = min(w1 - s.s0, s.ng);
+      if (i0 >= i1) continue;
+      // the item's 8 columns of q as B fragments
+      Query<C> q;
+      {
+        const bf16* qr = a.q + (int64_t)(s.row0 + g / a.share) * a.qs + (int64_t)(s.h * a.share + g % a.share) * D;
+        const bool has = g < s.rows;
+        if constexpr (C::QREG) {
 #pragma unroll
-      for (int i = tid; i < D; i += NT) {
-        const int col = i / (D / 8), ch = i % (D / 8);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (col < s.rows)
-          v = ldg_u4(a.q + (int64_t)(s.row0 + col / a.share) * a.qs + (int64_t)(s.h * a.share + col % a.share) * D + 8 * ch);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (C::BITS == 16)  // dims 16 ks + 8 half + 2t: lane t of chunk 2 ks + half
-            qs[(((ch >> 2) * 32) + 4 * col + e) * 4 + (ch & 3)] = w[e];
-          else  // octet o of a group: lane o % 4, half o / 4; pair e is k step e
-            qs[(((ch >> 3) * 2 + (e >> 1)) * 32 + 4 * col + (ch & 3)) * 4 + (e & 1) * 2 + ((ch >> 2) & 1)] = w[e];
-        }
-      }
-      __syncthreads();
-      const uint32_t qa = smem_u32(qs);
-      float xs[C::NG][2];
-      if constexpr (C::BITS == 4) {  // sums of q over the groups
-#pragma unroll
-        for (int gr = 0; gr < C::NG; ++gr) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          const uint32_t one = 0x3f803f80u;
-#pragma unroll
-          for (int k2 = 0; k2 < 2; ++k2) {
-            const uint4 q = lds128(qa + ((gr * 2 + k2) * 32 + lane) * 16);
-            mma16816(acc, one, one, one, one, q.x, q.y);
-            mma16816(acc, one, one, one, one, q.z, q.w);
+            for (int e = 0; e < 4; ++e) {
+              // bf16: k step 2i + e / 2, half e % 2: dims 16 ks + 8 half + 2t; 4-bit: k
+              // step 2i + e / 2 of group i / 2 is pair 2 (i % 2) + e / 2 of octets t, t + 4
+              const int d = C::BITS == 16 ? 32 * i + 8 * e + 2 * t
+                                          : 64 * (i >> 1) + 8 * (t + 4 * (e & 1)) + 2 * (2 * (i & 1) + (e >> 1));
+              w[e] = has ? __ldg(reinterpret_cast<const uint32_t*>(qr + d)) : 0u;
+            }
+            q.f[i] = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          xs[gr][0] = acc[0];
-          xs[gr][1] = acc[1];
+        } else {
+          uint32_t* qs = reinterpret_cast<uint32_t*>(sm + C::OFF_Q) + warp * 4 * D;
+          q.at = smem_u32(qs);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int d = 64 * (i >> 1) + 8 * (t + 4 * (e & 1)) + 2 * (2 * (i & 1) + (e >> 1));
+              qs[(i * 32 + lane) * 4 + e] = has ? __ldg(reinterpret_cast<const uint32_t*>(qr + d)) : 0u;
+            }
+          __syncwarp();
+        }
+        if constexpr (C::BITS == 4) {
+#pragma unroll
+          for (int gr = 0; gr < C::NG; ++gr) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t one = 0x3f803f80u;
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2) {
+              const uint4 f = q.frag(gr * 2 + k2, lane);
+              mma16816(acc, one, one, one, one, f.x, f.y);
+              mma16816(acc, one, one, one, one, f.z, f.w);
+            }
+            q.sum[gr][0] = acc[0];
+            q.sum[gr][1] = acc[1];
+          }
         }
       }
       Acc<C> x;
       reset<C>(x);
       const int pc0 = s.p0 + (2 * t) / a.share, pc1 = s.p0 + (2 * t + 1) / a.share;  // positions of the lane's columns
-      const int p1 = s.p0 + (s.rows - 1) / a.share;
+      const int pf = s.p0, p1 = s.p0 + (s.rows - 1) / a.share, low = s.low, hi = s.hi;
+      const int ns = s.ns, low_tile = s.low_tile;
 #pragma unroll 1
-      for (int i = s.i0 + warp; i < s.i1; i += NW) {
-        const int j0 = 16 * (i < s.ns ? i : s.low_tile + i - s.ns);
-        const int page = page_of(c, s.seq, j0 >> c.log_ps);
+      for (int i = i0; i < i1; ++i, ++gu) {
+        const int j0 = 16 * (i < ns ? i : low_tile + i - ns);
+        const bool here = (valid >> (gu & 31)) & 1;
+        const bool whole = here && j0 + 15 <= pf && (!a.window || j0 > p1 - a.window || j0 + 15 < a.sinks);
         float sc[4] = {0.f, 0.f, 0.f, 0.f};
+        uint8_t* piece = ring + (used % NP) * C::PIECE;
+        if constexpr (C::BITS == 16) {
 #pragma unroll
-        for (int hf = 0; hf < H; ++hf, ++used) {
+          for (int hf = 0; hf < H; ++hf, ++used) {
+            tc::pwait(&full[used % NP], (used / NP) & 1, failed, ws.status, 501);
+            scores<C>(smem_u32(ring + (used % NP) * C::PIECE), q, hf, lane, sc);
+            __syncwarp();  // every lane has read the piece
+            issue();
+          }
+        } else {
           tc::pwait(&full[used % NP], (used / NP) & 1, failed, ws.status, 501);
-          scores<C>(smem_u32(ring + (used % NP) * C::PIECE), qa, hf, xs, lane, sc);
-          __syncwarp();  // every lane has read the piece
-          issue();
+          scores<C>(smem_u32(piece), q, 0, lane, sc);
         }
-        const bool whole = page >= 0 && j0 + 15 <= s.p0 && (!a.window || j0 > p1 - a.window || j0 + 15 < a.sinks);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[e] *= a.sl;
-          if (!whole) {
+        for (int e = 0; e < 4; ++e) sc[e] *= a.sl;
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
             const int j = j0 + key_of<C>(g) + 8 * (e >> 1), p = e & 1 ? pc1 : pc0;
-            if (page < 0 || j > p || !(!a.window || j > p - a.window || j < a.sinks)) sc[e] = -INFINITY;
+            if (!here || j > p || !(!a.window || j > p - a.window || j < a.sinks)) sc[e] = -INFINITY;
           }
         }
         float mx[2] = {fmaxf(sc[0], sc[2]), fmaxf(sc[1], sc[3])};
@@ -552,38 +651,43 @@ __global__ void __launch_bounds__(C::NT, 1)
         const float p[4] = {ex2(sc[0] - r0), ex2(sc[1] - r1), ex2(sc[2] - r0), ex2(sc[3] - r1)};
         x.l[0] += p[0] + p[2];
         x.l[1] += p[1] + p[3];
-        uint32_t b0 = 0, b1 = 0;
-        if constexpr (C::BITS == 16) {
-          b0 = transpose8x8(pack_bf16x2(p[0], p[1]));
-          b1 = transpose8x8(pack_bf16x2(p[2], p[3]));
-        }
         // Rows that no row of the item sees can hold anything: zeros instead, since
         // a weight of zero times an infinity is no zero.
-        const bool seen = page >= 0 && j0 + 15 < s.hi && (j0 >= s.low || j0 + 15 < a.sinks);
-#pragma unroll
-        for (int hf = 0; hf < H; ++hf, ++used) {
-          tc::pwait(&full[used % NP], (used / NP) & 1, failed, ws.status, 502);
-          uint8_t* vp = ring + (used % NP) * C::PIECE;
-          if (!seen) {
+        const bool seen = whole || (here && j0 + 15 < hi && (j0 >= low || j0 + 15 < a.sinks));
+        auto blank = [&](uint8_t* vp) {
 #pragma unroll 1
-            for (int r = 0; r < 16; ++r) {
-              const int j = j0 + r;
-              if (page >= 0 && j < s.hi && (j >= s.low || j < a.sinks)) continue;
-              if constexpr (C::BITS == 16)
-                *reinterpret_cast<uint4*>(vp + (lane >> 3) * 2048 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-              else if (lane < C::NG)
-                *reinterpret_cast<uint32_t*>(vp + C::CODES + r * (D / 16) + lane * 4) = 0;
-            }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // before the copy that reuses the piece
-            __syncwarp();
+          for (int r = 0; r < 16; ++r) {
+            const int j = j0 + r;
+            if (here && j < hi && (j >= low || j < a.sinks)) continue;
+            if constexpr (C::BITS == 16)
+              *reinterpret_cast<uint4*>(vp + (lane >> 3) * 2048 + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+            else if (lane < C::NG)
+              *reinterpret_cast<uint32_t*>(vp + r * (D / 16) + lane * 4) = 0;
           }
-          add_values<C>(smem_u32(vp), hf, p, b0, b1, lane, x);
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // before the copy that reuses the piece
           __syncwarp();
+        };
+        if constexpr (C::BITS == 16) {
+          const uint32_t b0 = transpose8x8(pack_bf16x2(p[0], p[1])), b1 = transpose8x8(pack_bf16x2(p[2], p[3]));
+#pragma unroll
+          for (int hf = 0; hf < H; ++hf, ++used) {
+            tc::pwait(&full[used % NP], (used / NP) & 1, failed, ws.status, 502);
+            uint8_t* vp = ring + (used % NP) * C::PIECE;
+            if (!seen) blank(vp);
+            add_values<C>(smem_u32(vp), 0u, hf, p, b0, b1, lane, x);
+            __syncwarp();
+            issue();
+          }
+        } else {
+          if (!seen) blank(piece + 2 * C::CODES + C::PAIRS);
+          add_values<C>(smem_u32(piece) + C::CODES, smem_u32(piece) + 2 * C::CODES + C::PAIRS, 0, p, 0, 0, lane, x);
+          __syncwarp();
+          ++used;
           issue();
         }
       }
 
-      // -- join the warps.  Sums over keys: the lanes of a column (equal t)
+      // -- sums over keys: the lanes of a column (equal t)
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) {
         x.l[0] += __shfl_xor_sync(0xffffffffu, x.l[0], o);
@@ -595,128 +699,143 @@ __global__ void __launch_bounds__(C::NT, 1)
             x.corr[gr][1] += __shfl_xor_sync(0xffffffffu, x.corr[gr][1], o);
           }
       }
-      if (g == 0) {
-        ml[warp * 8 + 2 * t] = make_float2(x.m[0], x.l[0]);
-        ml[warp * 8 + 2 * t + 1] = make_float2(x.m[1], x.l[1]);
-      }
-      __syncthreads();  // the maxima are there; every warp is done with q
-      float f[2];
+      if constexpr (C::BITS == 4)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float M = -INFINITY;
+        for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w * 8 + 2 * t + e].x);
-        f[e] = x.m[e] == -INFINITY ? 0.f : ex2(x.m[e] - M);
-      }
-      float v[C::VPT];
+          for (int e = 0; e < 4; ++e) x.o[mt][e] += x.corr[mt >> 2][e & 1];
+      if (i0 == 0 && i1 == s.ng) {
+        const Rows r = {a.out, s.row0, s.rows, s.h * a.share, a.share, a.Hq};
+        const float v0 = x.l[0] == 0.f ? 0.f : 1.f / x.l[0], v1 = x.l[1] == 0.f ? 0.f : 1.f / x.l[1];
 #pragma unroll
-      for (int k = 0; k < C::VPT; ++k) v[k] = 0.f;
-#pragma unroll 1
-      for (int w0 = 0; w0 < NW; w0 += C::MW) {
-        if (warp >= w0 && warp < w0 + C::MW) {
-          float* ob = obuf + (warp - w0) * 8 * C::OS;
+        for (int mt = 0; mt < D / 16; ++mt)
+          store_tile<C>(r, mt, make_float4(x.o[mt][0], x.o[mt][1], x.o[mt][2], x.o[mt][3]), v0, v1, lane);
+      } else {
+        // a warp's part of its last item stays in its ring, which is done with
+        const int last = i1 == w1 - s.s0;
+        float4* po = reinterpret_cast<float4*>(wo);
 #pragma unroll
-          for (int mt = 0; mt < D / 16; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float add = C::BITS == 4 ? x.corr[C::BITS == 4 ? mt >> 2 : 0][e & 1] : 0.f;
-              // a warp without a key of this column has no say
-              ob[(2 * t + (e & 1)) * C::OS + dim_of<C>(mt, e, g)] = f[e & 1] == 0.f ? 0.f : (x.o[mt][e] + add) * f[e & 1];
-            }
+        for (int mt = 0; mt < D / 16; ++mt) {
+          const float4 v = make_float4(x.o[mt][0], x.o[mt][1], x.o[mt][2], x.o[mt][3]);
+          if (last)
+            reinterpret_cast<float4*>(ring)[mt * 32 + lane] = v;
+          else
+            __stcg(po + mt * 32 + lane, v);
         }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < C::VPT / 4; ++k) {
-          const int i = (k * NT + tid) * 4, row = i / D, d = i % D;
-#pragma unroll
-          for (int w = 0; w < C::MW; ++w) {
-            const float4 y = *reinterpret_cast<const float4*>(obuf + (w * 8 + row) * C::OS + d);
-            v[4 * k] += y.x;
-            v[4 * k + 1] += y.y;
-            v[4 * k + 2] += y.z;
-            v[4 * k + 3] += y.w;
-          }
+        if (g == 0) {
+          ml[(2 * warp + left) * 8 + 2 * t] = make_float2(x.m[0], x.l[0]);
+          ml[(2 * warp + left) * 8 + 2 * t + 1] = make_float2(x.m[1], x.l[1]);
         }
-        __syncthreads();
-      }
-#pragma unroll
-      for (int k = 0; k < C::VPT / 4; ++k) {
-        const int i = (k * NT + tid) * 4, row = i / D, d = i % D;
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w * 8 + row].x);
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const float2 y = ml[w * 8 + row];
-          if (y.x > -INFINITY) L += y.y * ex2(y.x - M);
-        }
-        if (!s.whole) {
-          *reinterpret_cast<float4*>(ws.o + ((int64_t)s.slot * 8 + row) * D + d) =
-              make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-          if (d == 0) ws.ml[s.slot * 8 + row] = make_float2(M, L);
-        } else if (row < s.rows) {
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          bf16* o = a.out + ((int64_t)(s.row0 + row / a.share) * a.Hq + s.h * a.share + row % a.share) * D + d;
-          *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v[4 * k] * inv, v[4 * k + 1] * inv),
-                                                    pack_bf16x2(v[4 * k + 2] * inv, v[4 * k + 3] * inv));
-        }
+        if (lane == 0) parts[2 * warp + left] = {s.item, s.row0, s.rows, s.h, s.cf, s.cl, s.slot, last};
+        ++left;
       }
     }
     if (n_seg < C::MAXSEG) break;
     done += n_seg;
+  }
+
+  // -- join the warps' parts: neighbours of one item form a group, [head, tail]
+  __syncthreads();
+  constexpr int NPART = 2 * NW;
+  if (tid < 8 * NPART) {  // the share of part k in column col; a part without a key of it has no say
+    const int k = tid >> 3, col = tid & 7, item = parts[k].item;
+    float f = 0.f, M = -INFINITY, L = 0.f;
+    if (item >= 0) {
+      for (int e = 0; e < NPART; ++e)
+        if (parts[e].item == item) M = fmaxf(M, ml[e * 8 + col].x);
+      for (int e = 0; e < NPART; ++e)
+        if (parts[e].item == item && ml[e * 8 + col].x > -INFINITY) L = fmaf(ex2(ml[e * 8 + col].x - M), ml[e * 8 + col].y, L);
+      if (ml[k * 8 + col].x > -INFINITY) f = ex2(ml[k * 8 + col].x - M);
+      bool tail = true;
+      for (int e = k + 1; e < NPART; ++e) tail &= parts[e].item != item;
+      if (tail) {
+        if (parts[k].cf != parts[k].cl) ws.ml[parts[k].slot * 8 + col] = make_float2(M, L);
+        tail_sh[k] = 1;
+      } else {
+        tail_sh[k] = 0;
+      }
+    } else {
+      tail_sh[k] = 0;
+    }
+    share_sh[k][col] = make_float2(f, L == 0.f ? 0.f : 1.f / L);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = tid; i < C::FRAGS; i += NT) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int k0 = 0; k0 < NPART; k0 += 8) {
+      float4 o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // a warp's first part is in scratch, its last one in its ring
+        const int k = k0 + e;
+        o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (parts[k].item >= 0)
+          o[e] = parts[k].in_ring ? reinterpret_cast<const float4*>(sm + (k >> 1) * (NP * C::PIECE))[i]
+                                  : __ldcg(reinterpret_cast<const float4*>(ws.wo) +
+                                           ((int64_t)blockIdx.x * NW + (k >> 1)) * 2 * D + i);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+          const int k = k0 + e;
+          const float2 s0 = share_sh[k][2 * t], s1 = share_sh[k][2 * t + 1];
+          v.x = s0.x == 0.f ? v.x : fmaf(s0.x, o[e].x, v.x);
+          v.y = s1.x == 0.f ? v.y : fmaf(s1.x, o[e].y, v.y);
+          v.z = s0.x == 0.f ? v.z : fmaf(s0.x, o[e].z, v.z);
+          v.w = s1.x == 0.f ? v.w : fmaf(s1.x, o[e].w, v.w);
+          if (tail_sh[k]) {
+            const Part r = parts[k];
+            if (r.cf == r.cl) {
+              const Rows rows = {a.out, r.row0, r.rows, r.h * a.share, a.share, a.Hq};
+              store_tile<C>(rows, i >> 5, v, s0.y, s1.y, lane);
+            } else {
+              reinterpret_cast<float4*>(ws.o)[(int64_t)r.slot * 2 * D + i] = v;
+            }
+            v = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+      }
+    }
   }
   // after a wait that gave up, no copy may land in the memory of a CTA that is gone
   if (*failed)
     for (int k = max(0, issued - NP); k < issued; ++k) tc::drain_wait(&full[k % NP], (k / NP) & 1);
 }
 
-// Joins the parts of the items that lie in several CTAs: block (q, row) the
-// item that ends in CTA q, a thread four dims.
-template <int D>
-__global__ void __launch_bounds__(D / 4) paged_attn_join_kernel(const AttnArgs a, const FewWs ws) {
-  __shared__ float w[kNumSMs], red[D / 128];
+// Joins the parts of the items that lie in several CTAs: block (q, y) 256
+// fragments of the item that ends in CTA q, a thread one.
+template <class C>
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, const FewWs ws) {
+  constexpr int D = C::D;
+  __shared__ float2 w[kNumSMs][8];  // (maximum, sum) of each part's columns
   griddep_wait();
-  const int q = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int q = blockIdx.x, tid = threadIdx.x, lane = tid & 31, t = lane & 3;
   const Split s = ws.split[q];
-  if (row >= s.rows) return;
+  if (s.rows == 0) return;
   const int n = q - s.cf + 1;
   auto slot = [&](int i) { return i == 0 ? s.first_slot : 2 * (s.cf + i); };
-  auto all = [&](float v, bool maxi) {  // over the block, the same in every thread
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float y = __shfl_xor_sync(0xffffffffu, v, o);
-      v = maxi ? fmaxf(v, y) : v + y;
-    }
-    __syncthreads();
-    if (lane == 0) red[tid >> 5] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int k = 1; k < D / 128; ++k) v = maxi ? fmaxf(v, red[k]) : v + red[k];
-    return v;
-  };
-  float M = -INFINITY, L = 0.f;
-  for (int i = tid; i < n; i += D / 4) M = fmaxf(M, w[i] = ws.ml[slot(i) * 8 + row].x);
-  M = all(M, true);
-  for (int i = tid; i < n; i += D / 4) {
-    const float f = w[i] == -INFINITY ? 0.f : ex2(w[i] - M);
-    w[i] = f;
-    if (f != 0.f) L += f * ws.ml[slot(i) * 8 + row].y;
+  for (int i = tid; i < 8 * n; i += 256) w[i >> 3][i & 7] = ws.ml[slot(i >> 3) * 8 + (i & 7)];
+  __syncthreads();
+  float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
+  for (int i = 0; i < n; ++i) {
+    M[0] = fmaxf(M[0], w[i][2 * t].x);
+    M[1] = fmaxf(M[1], w[i][2 * t + 1].x);
   }
-  L = all(L, false);  // its barriers also publish w
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int f = blockIdx.y * 256 + tid;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
   for (int i = 0; i < n; ++i) {
-    const float f = w[i];
-    const float4 o = *reinterpret_cast<const float4*>(ws.o + ((int64_t)slot(i) * 8 + row) * D + 4 * tid);
-    acc.x = fmaf(f, o.x, acc.x);
-    acc.y = fmaf(f, o.y, acc.y);
-    acc.z = fmaf(f, o.z, acc.z);
-    acc.w = fmaf(f, o.w, acc.w);
+    const float4 o = reinterpret_cast<const float4*>(ws.o)[(int64_t)slot(i) * 2 * D + f];
+    const float2 y0 = w[i][2 * t], y1 = w[i][2 * t + 1];
+    const float f0 = y0.x == -INFINITY ? 0.f : ex2(y0.x - M[0]), f1 = y1.x == -INFINITY ? 0.f : ex2(y1.x - M[1]);
+    L[0] = fmaf(f0, y0.y, L[0]);
+    L[1] = fmaf(f1, y1.y, L[1]);
+    v.x = fmaf(f0, o.x, v.x);
+    v.y = fmaf(f1, o.y, v.y);
+    v.z = fmaf(f0, o.z, v.z);
+    v.w = fmaf(f1, o.w, v.w);
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  bf16* o = a.out + ((int64_t)(s.row0 + row / a.share) * a.Hq + s.h * a.share + row % a.share) * D + 4 * tid;
-  *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  const Rows r = {a.out, s.row0, s.rows, s.h * a.share, a.share, a.Hq};
+  store_tile<C>(r, f >> 5, v, L[0] == 0.f ? 0.f : 1.f / L[0], L[1] == 0.f ? 0.f : 1.f / L[1], lane);
 }
 
 // Lane l's values l * P .. of row `slot` of a block.
@@ -803,6 +922,7 @@ size_t carve(void* base, const PagedDev& c, FewWs* w) {
   w->split = k.take<Split>(kNumSMs);
   w->o = k.take<float>((size_t)2 * kNumSMs * 8 * c.D);
   w->ml = k.take<float2>((size_t)2 * kNumSMs * 8);
+  w->wo = k.take<float>((size_t)Few<256, 4>::NW * kNumSMs * 8 * c.D);  // the most warps that a CTA has
   return align_up(k.off, 256);
 }
 
@@ -842,15 +962,15 @@ int launch_split(const PagedDev& c, const BatchDev& b, const AttnArgs& a, const 
   if (int rc = check_launch("paged_attn_split_kernel")) return rc;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(kNumSMs, kFewRows);
-  cfg.blockDim = dim3(C::D / 4);
+  cfg.gridDim = dim3(kNumSMs, C::FRAGS / 256);
+  cfg.blockDim = dim3(256);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   ProfScope prof_("paged_attn_join_kernel", st);
-  cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<C::D>, a, w);
+  cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<C>, a, w);
   return check_launch("paged_attn_join_kernel");
 }
 
