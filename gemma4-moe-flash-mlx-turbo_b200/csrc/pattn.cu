@@ -29,7 +29,8 @@ namespace pa {
 // An item inside one warp's part is written by it; parts of an item in several
 // warps are joined at the end of the CTA, parts in several CTAs by
 // paged_attn_join_kernel, in the order of the keys: no result depends on who
-// arrives first.
+// arrives first.  An item's beginning (its query, its first page ids) costs a
+// warp about as long as two granules do, so an item counts for kBegin more.
 //
 // One granule, with the 8 columns being the item's (row, head) pairs:
 //   S^T [16 keys x 8]   = K  [16 x D] Q^T    mma m16n8k16, A = K  (ldmatrix)
@@ -44,6 +45,8 @@ namespace pa {
 //   q . k = sum_g s_g (q . (128 + c))_g + (b_g - 128 s_g) (sum of q)_g
 // V's s goes into the weights, v = s (c - 8) + (b + 8 s), and what does not
 // depend on the dim is summed apart in fp32.
+
+constexpr int kBegin = 2;
 
 template <int D_, int BITS_>
 struct Few {
@@ -297,9 +300,12 @@ __device__ __forceinline__ void add_values(uint32_t vp, uint32_t pairs, int hf, 
 // Rows of the step that the item's columns are, for the stores.
 struct Rows {
   bf16* out;
-  int row0, rows, head0, share, Hq;
+  int row0, rows, head0, share, inv, Hq;
+  __device__ __forceinline__ Rows(const AttnArgs& a, int row0_, int rows_, int h)
+      : out(a.out), row0(row0_), rows(rows_), head0(h * a.share), share(a.share), inv(a.share_inv), Hq(a.Hq) {}
   __device__ __forceinline__ bf16* row(int col, int D) const {
-    return out + ((int64_t)(row0 + col / share) * Hq + head0 + col % share) * D;
+    const int i = (col * inv) >> 6;  // col / share
+    return out + ((int64_t)(row0 + i) * Hq + head0 + col - i * share) * D;
   }
 };
 
@@ -321,6 +327,19 @@ __device__ __forceinline__ void store_tile(const Rows& r, int mt, float4 v, floa
     if (2 * t < r.rows) *reinterpret_cast<uint32_t*>(r.row(2 * t, C::D) + d) = pack_bf16x2(v.x * i0, v.z * i0);
     if (2 * t + 1 < r.rows) *reinterpret_cast<uint32_t*>(r.row(2 * t + 1, C::D) + d) = pack_bf16x2(v.y * i1, v.w * i1);
   }
+}
+
+// Fragment i of a group of parts: to the output, or to the CTA's part of an item
+// that others hold too.  Out of line: it is called where code is unrolled.
+template <class C>
+__device__ __noinline__ void finish_group(const AttnArgs& a, const FewWs& ws, const Part& r, int i, float4 v, float i0,
+                                          float i1, int lane) {
+  if (r.cf != r.cl) {
+    reinterpret_cast<float4*>(ws.o)[(int64_t)r.slot * 2 * C::D + i] = v;
+    return;
+  }
+  const Rows rows(a, r.row0, r.rows, r.h);
+  store_tile<C>(rows, i >> 5, v, i0, i1, lane);
 }
 
 template <class C>
@@ -352,7 +371,7 @@ __global__ void __launch_bounds__(C::NT, 1)
 
   // What sequence k0 + tid has on the line, and the sums over the chunk's sequences.
   struct Mine {
-    int seq, first, count, p0, ng;   // table row, first row, rows, position of the first; granules of each of its items
+    int seq, first, count, p0, ng;   // table row, first row, rows, position of the first; length of each of its items
     int at_u, at_i, sum_u, sum_i;    // granules and sequences before it in the chunk, of the chunk
     Span sp;
   };
@@ -367,7 +386,7 @@ __global__ void __launch_bounds__(C::NT, 1)
       if (m.first >= 0 && m.count > 0 && m.count * (int64_t)a.share <= kFewRows) {
         m.p0 = len - m.count;
         m.sp = span_of<16>(m.p0, len - 1, a.window, a.sinks, capacity);
-        m.ng = max(1, m.sp.tiles);  // an item that sees nothing still has zeros to write
+        m.ng = max(1, m.sp.tiles) + kBegin;  // an item that sees nothing still has zeros to write
       }
     }
     int x = m.ng, y = m.ng > 0;
@@ -441,23 +460,24 @@ __global__ void __launch_bounds__(C::NT, 1)
         for (int h = (int)max((int64_t)0, -rel); h < c.Hkv; ++h) {
           const int64_t s0 = U + (int64_t)h * m.ng, at = rel + h;
           if (s0 >= u1 || at >= C::MAXSEG) break;
+          const int64_t r0 = s0 + kBegin, r1 = s0 + m.ng;  // its granules
           Seg s;
           s.seq = m.seq;
           s.h = h;
           s.row0 = m.first;
           s.rows = m.count * a.share;
           s.p0 = m.p0;
-          s.s0 = (int)(s0 - u0);
-          s.ng = m.ng;
+          s.s0 = (int)(r0 - u0);
+          s.ng = m.ng - kBegin;
           s.low = m.sp.low;
           s.hi = m.sp.hi;
           s.ns = m.sp.ns;
           s.low_tile = m.sp.low_tile;
           s.item = (int)(item0 + at);
-          s.cf = s0 >= u0 ? blockIdx.x : (int)(s0 / part);
-          s.cl = s0 + m.ng <= u1 ? blockIdx.x : (int)((s0 + m.ng - 1) / part);
-          s.slot = 2 * blockIdx.x + (s0 > u0);
-          s.first_slot = 2 * s.cf + (s0 > s.cf * part);
+          s.cf = r0 >= u0 && r0 < u1 ? blockIdx.x : (int)(r0 / part);
+          s.cl = r1 <= u1 ? blockIdx.x : (int)((r1 - 1) / part);
+          s.slot = 2 * blockIdx.x + (r0 > u0);
+          s.first_slot = 2 * s.cf + (r0 > s.cf * part);
           segs[at] = s;
           atomicMax(&seg_n, (int)at + 1);
         }
@@ -588,6 +608,15 @@ __global__ void __launch_bounds__(C::NT, 1)
           }
         }
       }
+      if (si + 1 < n_seg && segs[si + 1].s0 < w1) {  // the next item's query, while this one runs
+        const Seg& n = segs[si + 1];
+        if (g < n.rows) {
+          const bf16* nr = a.q + (int64_t)(n.row0 + g / a.share) * a.qs + (int64_t)(n.h * a.share + g % a.share) * D;
+#pragma unroll
+          for (int e = 0; e < D / 256; ++e)
+            asm volatile("prefetch.global.L1 [%0];\n" ::"l"(nr + 64 * (t + 4 * e)));
+        }
+      }
       Acc<C> x;
       reset<C>(x);
       const int pc0 = s.p0 + (2 * t) / a.share, pc1 = s.p0 + (2 * t + 1) / a.share;  // positions of the lane's columns
@@ -705,7 +734,7 @@ __global__ void __launch_bounds__(C::NT, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) x.o[mt][e] += x.corr[mt >> 2][e & 1];
       if (i0 == 0 && i1 == s.ng) {
-        const Rows r = {a.out, s.row0, s.rows, s.h * a.share, a.share, a.Hq};
+        const Rows r(a, s.row0, s.rows, s.h);
         const float v0 = x.l[0] == 0.f ? 0.f : 1.f / x.l[0], v1 = x.l[1] == 0.f ? 0.f : 1.f / x.l[1];
 #pragma unroll
         for (int mt = 0; mt < D / 16; ++mt)
@@ -739,25 +768,23 @@ __global__ void __launch_bounds__(C::NT, 1)
   constexpr int NPART = 2 * NW;
   if (tid < 8 * NPART) {  // the share of part k in column col; a part without a key of it has no say
     const int k = tid >> 3, col = tid & 7, item = parts[k].item;
-    float f = 0.f, M = -INFINITY, L = 0.f;
-    if (item >= 0) {
-      for (int e = 0; e < NPART; ++e)
-        if (parts[e].item == item) M = fmaxf(M, ml[e * 8 + col].x);
-      for (int e = 0; e < NPART; ++e)
-        if (parts[e].item == item && ml[e * 8 + col].x > -INFINITY) L = fmaf(ex2(ml[e * 8 + col].x - M), ml[e * 8 + col].y, L);
-      if (ml[k * 8 + col].x > -INFINITY) f = ex2(ml[k * 8 + col].x - M);
-      bool tail = true;
-      for (int e = k + 1; e < NPART; ++e) tail &= parts[e].item != item;
-      if (tail) {
-        if (parts[k].cf != parts[k].cl) ws.ml[parts[k].slot * 8 + col] = make_float2(M, L);
-        tail_sh[k] = 1;
-      } else {
-        tail_sh[k] = 0;
+    const float2 mine = ml[k * 8 + col];
+    float M = -INFINITY, L = 0.f;
+    bool tail = item >= 0;
+#pragma unroll
+    for (int e = 0; e < NPART; ++e)
+      if (parts[e].item == item) {
+        M = fmaxf(M, ml[e * 8 + col].x);
+        tail &= e <= k;
       }
-    } else {
-      tail_sh[k] = 0;
+#pragma unroll
+    for (int e = 0; e < NPART; ++e) {
+      const float2 y = ml[e * 8 + col];
+      if (parts[e].item == item && y.x > -INFINITY) L = fmaf(ex2(y.x - M), y.y, L);
     }
-    share_sh[k][col] = make_float2(f, L == 0.f ? 0.f : 1.f / L);
+    share_sh[k][col] = make_float2(item >= 0 && mine.x > -INFINITY ? ex2(mine.x - M) : 0.f, L == 0.f ? 0.f : 1.f / L);
+    tail_sh[k] = tail;
+    if (tail && parts[k].cf != parts[k].cl) ws.ml[parts[k].slot * 8 + col] = make_float2(M, L);
   }
   __syncthreads();
 #pragma unroll 1
@@ -777,22 +804,20 @@ __global__ void __launch_bounds__(C::NT, 1)
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-          const int k = k0 + e;
-          const float2 s0 = share_sh[k][2 * t], s1 = share_sh[k][2 * t + 1];
-          v.x = s0.x == 0.f ? v.x : fmaf(s0.x, o[e].x, v.x);
-          v.y = s1.x == 0.f ? v.y : fmaf(s1.x, o[e].y, v.y);
-          v.z = s0.x == 0.f ? v.z : fmaf(s0.x, o[e].z, v.z);
-          v.w = s1.x == 0.f ? v.w : fmaf(s1.x, o[e].w, v.w);
-          if (tail_sh[k]) {
-            const Part r = parts[k];
-            if (r.cf == r.cl) {
-              const Rows rows = {a.out, r.row0, r.rows, r.h * a.share, a.share, a.Hq};
-              store_tile<C>(rows, i >> 5, v, s0.y, s1.y, lane);
-            } else {
-              reinterpret_cast<float4*>(ws.o)[(int64_t)r.slot * 2 * D + i] = v;
-            }
-            v = make_float4(0.f, 0.f, 0.f, 0.f);
-          }
+        const int k = k0 + e;
+        const float2 s0 = share_sh[k][2 * t], s1 = share_sh[k][2 * t + 1];
+        if (s0.x != 0.f) {
+          v.x = fmaf(s0.x, o[e].x, v.x);
+          v.z = fmaf(s0.x, o[e].z, v.z);
+        }
+        if (s1.x != 0.f) {
+          v.y = fmaf(s1.x, o[e].y, v.y);
+          v.w = fmaf(s1.x, o[e].w, v.w);
+        }
+        if (tail_sh[k]) {
+          finish_group<C>(a, ws, parts[k], i, v, s0.y, s1.y, lane);
+          v = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
       }
     }
   }
@@ -834,7 +859,7 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
     v.z = fmaf(f0, o.z, v.z);
     v.w = fmaf(f1, o.w, v.w);
   }
-  const Rows r = {a.out, s.row0, s.rows, s.h * a.share, a.share, a.Hq};
+  const Rows r(a, s.row0, s.rows, s.h);
   store_tile<C>(r, f >> 5, v, L[0] == 0.f ? 0.f : 1.f / L[0], L[1] == 0.f ? 0.f : 1.f / L[1], lane);
 }
 
@@ -1017,7 +1042,7 @@ int fmoe_paged_attend(const fmoe_paged_kv_t* cache, int layer, const void* q, in
   pa::FewWs w;
   pa::carve(workspace, c, &w);
   const int share = q_heads / c.Hkv;
-  const pa::AttnArgs a = {static_cast<const bf16*>(q), static_cast<bf16*>(out), q_stride, q_heads, share, layer,
+  const pa::AttnArgs a = {static_cast<const bf16*>(q), static_cast<bf16*>(out), q_stride, q_heads, share, 64 / share + 1, layer,
                           std::min(window, 1 << 30), std::min(sinks, 1 << 30), scale * 1.4426950408889634f};
   if (c.D == 256)
     rc = c.bits == 16 ? pa::launch_split<pa::Few<256, 16>>(c, b, a, w, st) : pa::launch_split<pa::Few<256, 4>>(c, b, a, w, st);

@@ -10,7 +10,8 @@ struct AttnArgs {
   const bf16* q;  // [tokens][Hq][D], rows qs values apart
   bf16* out;      // [tokens][Hq][D]
   int64_t qs;
-  int Hq, share, layer, window, sinks;  // share: query heads of a kv head
+  int Hq, share, share_inv;  // share: query heads of a kv head; (x * share_inv) >> 6 is x / share for x < 8
+  int layer, window, sinks;
   float sl;                             // scale * log2(e): weights are powers of two
 };
 
