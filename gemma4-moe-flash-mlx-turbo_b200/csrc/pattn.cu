@@ -1012,7 +1012,9 @@ size_t fmoe_paged_attend_workspace_bytes(const fmoe_paged_kv_t* cache, int q_hea
   if (paged_to_dev(cache, &c, false) || q_heads < 1 || q_heads % c.Hkv || q_heads / c.Hkv > 8 || n < 0 || tokens < 0)
     return 0;
   pa::FewWs w;
-  return pa::carve(nullptr, c, &w);
+  const size_t few = pa::carve(nullptr, c, &w);  // the two kernels' scratch is used in turn
+  const int share = q_heads / c.Hkv;
+  return (int64_t)max_new * share <= pa::kFewRows ? few : std::max(few, pa::tile_workspace_bytes(share, tokens, n));
 }
 
 int fmoe_paged_attend(const fmoe_paged_kv_t* cache, int layer, const void* q, int64_t q_stride, int q_heads,
@@ -1049,6 +1051,7 @@ int fmoe_paged_attend(const fmoe_paged_kv_t* cache, int layer, const void* q, in
   else
     rc = c.bits == 16 ? pa::launch_split<pa::Few<512, 16>>(c, b, a, w, st) : pa::launch_split<pa::Few<512, 4>>(c, b, a, w, st);
   if (rc || (int64_t)b.max_new * share <= pa::kFewRows) return rc;
+  if (c.bits == 16) return pa::launch_tiles(c, b, a, workspace, st);
   ProfScope prof_("paged_attn_rows_kernel", st);
   const dim3 grid((unsigned)b.tokens, (unsigned)q_heads);
   if (c.D == 256)

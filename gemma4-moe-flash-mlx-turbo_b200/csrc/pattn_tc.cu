@@ -1,0 +1,695 @@
+// Attention over the pages of a cache for sequences with many new rows:
+// prompts, chunks of prompts, verified drafts.  Bound by the tensor cores.
+//
+// An item is a tile of up to 128 (row, query head of the kv head's group) pairs
+// of one sequence, token-major, against the keys that some row of it sees, 64 at
+// a time; for 512 dims also one of the two halves of the output's dims (an
+// output of 128 rows x 512 fp32 would fill tensor memory, so both halves compute
+// the scores).  All items' key tiles form one line that the CTAs cut evenly; an
+// item cut by a boundary leaves parts that paged_attn_tile_join_kernel joins.
+//
+// Tensor memory (512 columns): O 256 | Q (256 dims, bf16 pairs) 128 | S 2 x 64.
+//   S_j = Q K_j^T     A = Q from tensor memory (dims past 256: shared memory), B = K_j, K-major
+//   O  += P_j V_j     A = P_j from tensor memory, over S_j's columns, B = V_j as it lies, MN-major
+// With Q and P in tensor memory an instruction reads only B from shared memory,
+// 64 bytes a clock; from shared memory A alone would ask for all of its 128.
+// The issue order S_{j+1}, O += P_j V_j lets the softmax of a tile run under the
+// products of its neighbours.  Weights are bf16 (their sum is of the unrounded
+// ones); O is rescaled, by the softmax's warps, only when a row's maximum passes
+// the one in use by 2^8.
+//
+// Warps: 0 copies (TMA, 16..64 rows of 64 dims a box, a box in one page),
+// 1 issues the products, 4..7 softmax, output and Q.
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+#include "pattn.cuh"
+#include "tc.cuh"
+
+namespace fmoe {
+namespace pa {
+
+constexpr int kTile = 64;     // keys of a tile
+constexpr int kTileBegin = 2; // an item's beginning and end, in tiles of its time
+constexpr int kUnit = 32768;  // bytes of a ring unit: 64 keys x 256 dims
+
+template <int D_>
+struct Tile {
+  static constexpr int D = D_, HALVES = D / 256, KU = D / 256;  // KU: units of a K tile
+  static constexpr int NU = D == 256 ? 6 : 5;
+  static constexpr int OFF_Q = NU * kUnit;  // dims 256.. of Q, 4 blocks of [128 rows][128 bytes], swizzled
+  static constexpr int OFF_BAR = OFF_Q + (D == 512 ? 65536 : 0);
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static_assert(SMEM <= 227 * 1024 - 256, "shared memory");
+};
+
+// A tile of rows: what every kv head (and half) does with it.
+struct RowTile {
+  int seq, row0, tokens, p0;  // table row, first row of the step, its rows, position of the first
+  int low, hi, ns, low_tile;  // Span in tiles of 64
+  int64_t before;             // key tiles (with kTileBegin each) of the row tiles before it
+  int tiles, pad;
+};
+static_assert(sizeof(RowTile) == 48, "row tile list");
+
+struct TileSplit {  // an item that ends in a CTA and began in an earlier one
+  int row0, rows, h, half, cf, first_slot, pad[2];
+};
+struct TileWs {
+  int* status;
+  int64_t* total;    // [2] key tiles of all row tiles; their number
+  RowTile* list;     // [cap]
+  int64_t cap;
+  TileSplit* split;  // [grid]
+  float* o;          // [2 * grid][128][256]
+  float2* ml;        // [2 * grid][128]
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+
+// D += A (tensor memory) . B (shared memory descriptor)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// V as B, rows of keys with the dims together (MN-major): 64-dim blocks of
+// [64 keys][128 bytes] 8 KB apart (leading offset), 8-key groups 1 KB apart.
+__device__ __forceinline__ uint64_t v_desc(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+constexpr uint32_t kBMajorMN = 1u << 16;
+
+__device__ __forceinline__ int64_t scan64(int64_t v, int64_t* sh, int64_t* total) {  // exclusive, 1024 threads
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) sh[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t w = sh[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    sh[lane] = w;
+  }
+  __syncthreads();
+  *total = sh[31];
+  return (warp ? sh[warp - 1] : 0) + x - v;
+}
+
+// The list of row tiles of the sequences with more than kFewRows pairs, and how
+// many key tiles come before each.
+__global__ void __launch_bounds__(1024) paged_attn_plan_kernel(PagedDev c, BatchDev b, AttnArgs a, TileWs ws) {
+  __shared__ int64_t sh[32];
+  __shared__ int at[1024], count_sh[1024], first_sh[1024], len_sh[1024];
+  const int tid = threadIdx.x, TT = 128 / a.share;
+  const int capacity = c.max_blocks << c.log_ps;
+  griddep_launch_dependents();
+  int64_t listed = 0, before = 0;
+  for (int k0 = 0; k0 < b.n; k0 += 1024) {
+    const int k = k0 + tid;
+    int first = 0, count = 0, len = 0, nt = 0;
+    if (k < b.n) {
+      first = b.q_start[k];
+      count = (int)min((int64_t)b.q_start[k + 1], b.tokens) - first;
+      len = b.kv_len[k];
+      if (first >= 0 && count > 0 && count * (int64_t)a.share > kFewRows) nt = (count + TT - 1) / TT;
+    }
+    int64_t sum;
+    at[tid] = (int)scan64(nt, sh, &sum);
+    sum = min(sum, ws.cap - listed);  // rows that several sequences claim are the caller's mistake, not ours to follow
+    count_sh[tid] = count;
+    first_sh[tid] = first;
+    len_sh[tid] = len;
+    __syncthreads();
+    for (int64_t i0 = 0; i0 < sum; i0 += 1024) {
+      const int i = (int)i0 + tid;
+      RowTile r = {};
+      if (i < sum) {
+        int lo = 0, hi = min(1024, b.n - k0) - 1;  // the last sequence whose tiles begin at or before i
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (at[mid] <= i)
+            lo = mid;
+          else
+            hi = mid - 1;
+        }
+        const int t0 = (i - at[lo]) * TT;
+        r.seq = b.seqs[k0 + lo];
+        r.row0 = first_sh[lo] + t0;
+        r.tokens = min(TT, count_sh[lo] - t0);
+        r.p0 = len_sh[lo] - count_sh[lo] + t0;
+        const Span s = span_of<kTile>(r.p0, r.p0 + r.tokens - 1, a.window, a.sinks, capacity);
+        r.low = s.low;
+        r.hi = s.hi;
+        r.ns = s.ns;
+        r.low_tile = s.low_tile;
+        r.tiles = max(1, s.tiles);  // a tile that sees nothing still has zeros to write
+      }
+      int64_t more;
+      const int64_t p = scan64(i < sum ? r.tiles + kTileBegin : 0, sh, &more);
+      r.before = before + p;
+      if (i < sum) ws.list[listed + i] = r;
+      before += more;
+    }
+    listed += sum;
+    __syncthreads();
+  }
+  if (tid == 0) {
+    ws.total[0] = before;
+    ws.total[1] = listed;
+  }
+}
+
+// Walks a CTA's items: its stretch [u0, u1) of the line, which is the row tiles'
+// key tiles once for every (half, kv head).
+struct Walk {
+  int64_t u, u1, total, count, i;  // where it is; the row tile
+  int hh;                          // half * Hkv + kv head
+  RowTile r;
+  int k0, k1;    // key tiles of the item in this stretch
+  int64_t s0;    // where the item's key tiles begin on the line
+  __device__ __forceinline__ bool load(const TileWs& ws) {  // false: the stretch is done
+    for (;;) {
+      if (u >= u1) return false;
+      if (i >= count) {
+        i = 0;
+        ++hh;
+      }
+      const int4* p = reinterpret_cast<const int4*>(ws.list + i);
+      reinterpret_cast<int4*>(&r)[0] = __ldcg(p);
+      reinterpret_cast<int4*>(&r)[1] = __ldcg(p + 1);
+      reinterpret_cast<int4*>(&r)[2] = __ldcg(p + 2);
+      s0 = hh * total + r.before + kTileBegin;
+      k0 = (int)max(u - s0, (int64_t)0);
+      k1 = (int)min(u1 - s0, (int64_t)r.tiles);
+      if (k0 < k1) return true;
+      next();
+    }
+  }
+  __device__ __forceinline__ void next() {
+    u = s0 + r.tiles;
+    ++i;
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(256, 1)
+    paged_attn_tile_kernel(const __grid_constant__ CUtensorMap map, const PagedDev c, const AttnArgs a, const TileWs ws) {
+  using C = Tile<D>;
+  constexpr int NU = C::NU, KU = C::KU;
+  extern __shared__ uint8_t sm_raw[];
+  __shared__ uint32_t tmem_sh;
+  __shared__ int failed_sh;
+  uint8_t* sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+  uint64_t* empty = full + NU;
+  uint64_t* s_full = empty + NU;    // [2]
+  uint64_t* p_full = s_full + 2;    // [2]
+  uint64_t* pv_done = p_full + 2;   // [2]: the scores of tile j are in after the product of tile j - 2
+  uint64_t* q_full = pv_done + 2;
+  uint64_t* o_free = q_full + 1;
+  volatile int* failed = &failed_sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < NU; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(q_full, 4);
+    mbar_init(o_free, 4);
+    failed_sh = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_sh)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  griddep_launch_dependents();
+  griddep_wait();  // the list
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = tmem_sh, tO = tmem, tQ = tmem + 256, tS = tmem + 384;
+
+  Walk w;
+  w.total = __ldcg(reinterpret_cast<const long long*>(ws.total));
+  w.count = __ldcg(reinterpret_cast<const long long*>(ws.total) + 1);
+  const int64_t line = w.total * c.Hkv * C::HALVES;
+  const int64_t part = max((int64_t)4, (line + gridDim.x - 1) / gridDim.x);
+  const int64_t u0 = min(line, blockIdx.x * part);
+  w.u = u0;
+  w.u1 = min(line, u0 + part);
+  const bool any = u0 < w.u1;
+  if (any) {  // the row tile that the stretch begins in: a 256-way search
+    w.hh = (int)(u0 / w.total);
+    const int64_t r = u0 - w.hh * w.total;
+    int64_t lo = 0, n = w.count;
+    while (n > 1) {
+      const int64_t step = (n + 255) / 256, k = lo + tid * step;
+      const int hits = __syncthreads_count(tid * step < n && __ldcg(reinterpret_cast<const long long*>(&ws.list[min(k, w.count - 1)].before)) <= r);
+      lo += (hits - 1) * step;
+      n = min(step, w.count - lo);
+      if (step == 1) break;
+    }
+    w.i = lo;
+  }
+  if (tid == 0) ws.split[blockIdx.x].rows = 0;
+  __syncthreads();
+
+  if (any && warp == 0) {
+    // ---- copies: K_0, then K_{j+1}, V_j
+    const int box = min(c.ps, kTile), per = kTile / box;  // rows of a box, boxes of a unit's block
+    int n = 0;
+    while (w.load(ws)) {
+      const int h = w.hh % c.Hkv, half = w.hh / c.Hkv;
+      int entry = -1, entry0 = -64;  // lanes hold the pages of 32 boxes
+      auto copy = [&](int k, int which, int xd) {  // unit of tile k: dims xd .. xd + 255
+        const int s = n % NU;
+        if (n >= NU) tc::pwait(&empty[s], ((n / NU) - 1) & 1, failed, ws.status, 601);
+        const int b0 = k * per;
+        if (b0 < entry0 || b0 + per > entry0 + 32) {
+          entry0 = b0;
+          const int j = b0 + lane, kt = j / per, tile = kt < w.r.ns ? kt : w.r.low_tile + kt - w.r.ns;
+          entry = kt < w.k1 ? page_of(c, w.r.seq, ((int64_t)tile * kTile + (j % per) * box) >> c.log_ps) : -1;
+        }
+        const int gr = min(lane >> 2, per - 1), cb = lane & 3;
+        const int page = __shfl_sync(0xffffffffu, entry, b0 + gr - entry0);
+        const int tile = k < w.r.ns ? k : w.r.low_tile + k - w.r.ns;
+        const int slot = (tile * kTile + gr * box) & (c.ps - 1);
+        // a page that is missing is read past the end: zeros
+        const int y = page >= 0 ? ((page * c.Hkv + h) * 2 + which) * c.ps + slot : 2 * c.num_pages * c.Hkv * c.ps;
+        if (!__any_sync(0xffffffffu, *failed)) {
+          if (lane == 0) mbar_arrive_expect_tx(&full[s], kUnit);
+          __syncwarp();
+          if (lane < 4 * per) tc::tma2d(sm + s * kUnit + cb * 8192 + gr * box * 128, &map, xd + 64 * cb, y, &full[s]);
+          ++n;
+        }
+      };
+      auto copy_k = [&](int k) {
+#pragma unroll
+        for (int d = 0; d < KU; ++d) copy(k, 0, 256 * d);
+      };
+      copy_k(w.k0);
+#pragma unroll 1
+      for (int k = w.k0; k < w.k1; ++k) {
+        if (k + 1 < w.k1) copy_k(k + 1);
+        copy(k, 1, 256 * half);
+      }
+      w.next();
+    }
+    // every copy issued lands before the CTA ends
+    for (int k = max(0, n - NU); k < n; ++k) tc::drain_wait(&full[k % NU], (k / NU) & 1);
+  } else if (any && warp == 1) {
+    // ---- products
+    if (lane == 0) {
+      const uint32_t id_s = tc::idesc_n(kTile), id_o = tc::idesc_n(256) | kBMajorMN;
+      int n = 0, g = 0, item = 0;  // units, tiles, items so far
+      while (w.load(ws)) {
+        auto scores = [&](int j) {  // S_j of the item's tile j (j-th here)
+          const uint32_t d = tS + ((g + j) & 1) * kTile;
+#pragma unroll
+          for (int u = 0; u < KU; ++u, ++n) {
+            const int s = n % NU;
+            tc::pwait(&full[s], (n / NU) & 1, failed, ws.status, 602);
+            tc::tc_fence_after();
+            const uint32_t kb = smem_u32(sm + s * kUnit);
+#pragma unroll
+            for (int ks = 0; ks < 16; ++ks) {
+              const uint64_t bd = tc::sw128_desc(kb + (ks >> 2) * 8192 + (ks & 3) * 32);
+              if (u == 0)
+                mma_ts(d, tQ + 8 * ks, bd, id_s, ks > 0);
+              else
+                tc::mma_ss(d, tc::sw128_desc(smem_u32(sm + C::OFF_Q) + (ks >> 2) * 16384 + (ks & 3) * 32), bd, id_s, 1);
+            }
+            tc::mma_commit(&empty[s]);
+          }
+          tc::mma_commit(&s_full[(g + j) & 1]);
+        };
+        const int tiles = w.k1 - w.k0;
+        tc::pwait(q_full, item & 1, failed, ws.status, 603);
+        tc::tc_fence_after();
+        scores(0);
+#pragma unroll 1
+        for (int j = 0; j < tiles; ++j) {
+          if (j + 1 < tiles) scores(j + 1);
+          tc::pwait(&p_full[(g + j) & 1], ((g + j) >> 1) & 1, failed, ws.status, 604);
+          if (j == 0 && item > 0) tc::pwait(o_free, (item - 1) & 1, failed, ws.status, 605);
+          const int s = n % NU;
+          tc::pwait(&full[s], (n / NU) & 1, failed, ws.status, 606);
+          tc::tc_fence_after();
+          const uint32_t vb = smem_u32(sm + s * kUnit), p = tS + ((g + j) & 1) * kTile;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) mma_ts(tO, p + 8 * kk, v_desc(vb + kk * 2048), id_o, j > 0 || kk > 0);
+          tc::mma_commit(&empty[s]);
+          tc::mma_commit(&pv_done[(g + j) & 1]);
+          ++n;
+          if (*failed) break;
+        }
+        g += tiles;
+        ++item;
+        w.next();
+        if (*failed) break;
+      }
+      // the products in flight end before the CTA does (a failure may have left some barrier short)
+      if (g > 0) tc::drain_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
+    }
+  } else if (any && warp >= 4) {
+    // ---- softmax: a thread is a row
+    const int qw = warp & 3, row = qw * 32 + lane;
+    const uint32_t lane_at = (uint32_t)(qw * 32) << 16;
+    int g = 0, item = 0, units = 0;
+    int tok, col;  // the row's token of the tile, its head of the group
+    tok = row / a.share;
+    col = row - tok * a.share;
+    auto load_q = [&]() {  // this row of Q: dims 0 .. 255 to tensor memory, the others to shared memory
+      const int h = w.hh % c.Hkv;
+      const bool has = tok < w.r.tokens;
+      const bf16* q = a.q + (int64_t)(w.r.row0 + tok) * a.qs + (int64_t)(h * a.share + col) * D;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {  // 64 dims
+        uint32_t r[32];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint4 v = has ? ldg_u4(q + 64 * i + 8 * e) : make_uint4(0, 0, 0, 0);
+          r[4 * e] = v.x, r[4 * e + 1] = v.y, r[4 * e + 2] = v.z, r[4 * e + 3] = v.w;
+        }
+        tmem_st32(tQ + lane_at + 32 * i, r);
+      }
+      if constexpr (D == 512) {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint4 v = has ? ldg_u4(q + 256 + 64 * i + 8 * e) : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(sm + C::OFF_Q + i * 16384 + row * 128 + ((e ^ (row & 7)) << 4)) = v;
+          }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      }
+      tmem_st_wait();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    };
+    bool more = w.load(ws);
+    if (more) load_q();
+    while (more) {
+      const RowTile r = w.r;
+      const int k0 = w.k0, k1 = w.k1, h = w.hh % c.Hkv, half = w.hh / c.Hkv, tiles = k1 - k0;
+      const int64_t s0 = w.s0;
+      const int p = r.p0 + min(tok, r.tokens - 1), pl = r.p0 + r.tokens - 1;  // the row's position, the last row's
+      float m = -INFINITY, l = 0.f;
+      int entry = -1, entry0 = -64;  // lanes hold the pages of 8 tiles' 16-key granules
+#pragma unroll 1
+      for (int j = 0; j < tiles; ++j) {
+        const int k = k0 + j, j0 = kTile * (k < r.ns ? k : r.low_tile + k - r.ns);
+        if (k >= entry0 + 8) {
+          entry0 = k;
+          const int kt = k + (lane >> 2), tile = kt < r.ns ? kt : r.low_tile + kt - r.ns;
+          entry = kt < k1 ? page_of(c, r.seq, ((int64_t)tile * kTile + 16 * (lane & 3)) >> c.log_ps) : -1;
+        }
+        const uint32_t here = (__ballot_sync(0xffffffffu, entry >= 0) >> (4 * (k - entry0))) & 15;
+        const bool whole = here == 15 && j0 + kTile - 1 <= r.p0 && (!a.window || j0 > pl - a.window || j0 + kTile - 1 < a.sinks);
+        const uint32_t tSj = tS + lane_at + ((g + j) & 1) * kTile;
+        tc::pwait(&s_full[(g + j) & 1], ((g + j) >> 1) & 1, failed, ws.status, 607);
+        tc::tc_fence_after();
+        float s[2][32];
+        tmem_ld32(tSj, s[0]);
+        tmem_ld32(tSj + 32, s[1]);
+        tc::tmem_ld_wait();
+        // the scale is part of the exponent's fma, except where scores are masked
+        // (or it is not positive, and a maximum would not pass through it)
+        float mul = a.sl;
+        if (!whole || !(a.sl > 0.f)) {
+          mul = 1.f;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            const int jj = j0 + i;
+            const bool see = ((here >> (i >> 4)) & 1) && jj <= p && (!a.window || jj > p - a.window || jj < a.sinks);
+            s[i >> 5][i & 31] = see ? s[i >> 5][i & 31] * a.sl : -INFINITY;
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i >> 5][i & 31]);
+        const float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+        if (__any_sync(0xffffffffu, best > m + 8.f)) {
+          const float mn = fmaxf(m, best), f = m == mn ? 1.f : ex2(m - mn);
+          m = mn;
+          l *= f;
+          if (j > 0) {
+            tc::pwait(&pv_done[(g + j - 1) & 1], ((g + j - 1) >> 1) & 1, failed, ws.status, 608);
+            tc::tc_fence_after();
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+              float o[32];
+              uint32_t u[32];
+              tmem_ld32(tO + lane_at + 32 * i, o);
+              tc::tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(o[e] * f);
+              tmem_st32(tO + lane_at + 32 * i, u);
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        uint32_t pk[32];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float x = s[i >> 4][(2 * i) & 31], y = s[i >> 4][(2 * i + 1) & 31];
+          x = ex2(fmaf(x, mul, -ref));
+          y = ex2(fmaf(y, mul, -ref));
+          sum[i & 3] += x + y;
+          pk[i] = pack_bf16x2(x, y);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st32(tSj, pk);
+        // Rows of V that no row of the tile sees can hold anything: zeros instead
+        const bool seen = whole || (here == 15 && j0 + kTile - 1 < r.hi && (j0 >= r.low || j0 + kTile - 1 < a.sinks));
+        if (!seen) {
+          const int n = units + KU * min(j + 2, tiles) + j, sv = n % NU;  // V_j's unit
+          tc::pwait(&full[sv], (n / NU) & 1, failed, ws.status, 609);
+          uint8_t* vb = sm + sv * kUnit;
+          const int t4 = tid & 127;  // a key per pair of threads, 2 of the 4 blocks each
+          const int jj = j0 + (t4 >> 1);
+          if (!(((here >> (t4 >> 5)) & 1) && jj < r.hi && (jj >= r.low || jj < a.sinks))) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              *reinterpret_cast<uint4*>(vb + ((t4 & 1) * 2 + (e >> 3)) * 8192 + (t4 >> 1) * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        }
+        tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[(g + j) & 1]);
+        if (__any_sync(0xffffffffu, *failed)) break;
+      }
+      units += (KU + 1) * tiles;
+      // the next item's Q before this one's output: its first scores run meanwhile
+      tc::pwait(&pv_done[(g + tiles - 1) & 1], ((g + tiles - 1) >> 1) & 1, failed, ws.status, 610);
+      tc::tc_fence_after();
+      g += tiles;
+      w.next();
+      more = !*failed && w.load(ws);
+      more = __all_sync(0xffffffffu, more);
+      if (more) load_q();
+      const int64_t e0 = s0, e1 = s0 + r.tiles;  // the item on the line
+      const int cf = e0 >= u0 ? (int)blockIdx.x : (int)(e0 / part), cl = e1 <= w.u1 ? (int)blockIdx.x : (int)((e1 - 1) / part);
+      const bool has = tok < r.tokens && row < 128 / a.share * a.share;
+      if (cf == cl) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        bf16* o = a.out + ((int64_t)(r.row0 + tok) * a.Hq + h * a.share + col) * D + 256 * half;
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          float v[32];
+          tmem_ld32(tO + lane_at + 32 * i, v);
+          tc::tmem_ld_wait();
+          if (has)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(o + 32 * i + 8 * e) =
+                  make_uint4(pack_bf16x2(v[8 * e] * inv, v[8 * e + 1] * inv), pack_bf16x2(v[8 * e + 2] * inv, v[8 * e + 3] * inv),
+                             pack_bf16x2(v[8 * e + 4] * inv, v[8 * e + 5] * inv), pack_bf16x2(v[8 * e + 6] * inv, v[8 * e + 7] * inv));
+        }
+      } else {
+        const int slot = 2 * blockIdx.x + (e0 > u0);
+        float* o = ws.o + ((int64_t)slot * 128 + row) * 256;
+        ws.ml[slot * 128 + row] = make_float2(m, l);
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          float v[32];
+          tmem_ld32(tO + lane_at + 32 * i, v);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(o + 32 * i + 4 * e) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+        }
+        if (cf < (int)blockIdx.x && cl == (int)blockIdx.x && row == 0) {
+          TileSplit* t = ws.split + blockIdx.x;
+          t->row0 = r.row0;
+          t->rows = r.tokens * a.share;
+          t->h = h;
+          t->half = half;
+          t->cf = cf;
+          t->first_slot = 2 * cf + (e0 > cf * part);
+        }
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free);
+      ++item;
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// Joins the parts of the items that lie in several CTAs: block (q, y) rows 8y ..
+// of the item that ends in CTA q, a warp a row, a lane 8 dims.
+__global__ void __launch_bounds__(256) paged_attn_tile_join_kernel(const AttnArgs a, const TileWs ws, int D) {
+  griddep_wait();
+  const int q = blockIdx.x, row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const TileSplit s = ws.split[q];
+  if (row >= s.rows) return;
+  const int n = q - s.cf + 1;
+  auto slot = [&](int i) { return (int64_t)(i == 0 ? s.first_slot : 2 * (s.cf + i)) * 128 + row; };
+  float M = -INFINITY, L = 0.f, v[8] = {};
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, ws.ml[slot(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float2 y = ws.ml[slot(i)];
+    const float4* o = reinterpret_cast<const float4*>(ws.o + slot(i) * 256 + 8 * lane);
+    const float4 x0 = o[0], x1 = o[1];
+    const float f = y.x == -INFINITY ? 0.f : ex2(y.x - M);
+    L = fmaf(f, y.y, L);
+    const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fmaf(f, x[e], v[e]);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int tok = row / a.share, col = row - tok * a.share;
+  bf16* o = a.out + ((int64_t)(s.row0 + tok) * a.Hq + s.h * a.share + col) * D + 256 * s.half + 8 * lane;
+  *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
+                                            pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
+}
+
+size_t carve_tile(void* base, int share, int64_t tokens, int64_t n, TileWs* w) {
+  Carver k(base);
+  w->status = k.take<int>(64);  // the workspace's status word: the one that the split kernel has
+  w->total = k.take<int64_t>(2);
+  w->cap = tokens / (128 / share) + n + 1;
+  w->list = k.take<RowTile>((size_t)w->cap);
+  w->split = k.take<TileSplit>(kNumSMs);
+  w->o = k.take<float>((size_t)2 * kNumSMs * 128 * 256);
+  w->ml = k.take<float2>((size_t)2 * kNumSMs * 128);
+  return align_up(k.off, 256);
+}
+
+size_t tile_workspace_bytes(int share, int64_t tokens, int64_t n) {
+  TileWs w;
+  return carve_tile(nullptr, share, tokens, n, &w);
+}
+
+template <class K>
+static int launch_pdl(const char* name, cudaStream_t st, dim3 grid, int threads, size_t smem, const K& go) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  ProfScope prof_(name, st);
+  go(&cfg);
+  return check_launch(name);
+}
+
+template <int D>
+static int launch_tiles_d(const PagedDev& c, const BatchDev& b, const AttnArgs& a, const TileWs& w, cudaStream_t st) {
+  static std::once_flag once;
+  static cudaError_t err = cudaSuccess;
+  std::call_once(once, [] {
+    err = cudaFuncSetAttribute(paged_attn_tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<D>::SMEM);
+  });
+  if (err != cudaSuccess)
+    return set_error(FMOE_ERR_CUDA, "paged_attend: shared memory attribute: %s", cudaGetErrorString(err));
+  const int64_t rows = 2ll * c.num_pages * c.Hkv * c.ps;
+  CUtensorMap map;
+  const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)D * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)std::min(c.ps, kTile)};
+  if (int rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c.pages + a.layer * c.layer, dims, strides, box,
+                      CU_TENSOR_MAP_SWIZZLE_128B, "pages"))
+    return rc;
+  {
+    ProfScope prof_("paged_attn_plan_kernel", st);
+    paged_attn_plan_kernel<<<1, 1024, 0, st>>>(c, b, a, w);
+  }
+  if (int rc = check_launch("paged_attn_plan_kernel")) return rc;
+  if (int rc = launch_pdl("paged_attn_tile_kernel", st, dim3(kNumSMs), 256, Tile<D>::SMEM, [&](cudaLaunchConfig_t* cfg) {
+        cudaLaunchKernelEx(cfg, paged_attn_tile_kernel<D>, map, c, a, w);
+      }))
+    return rc;
+  return launch_pdl("paged_attn_tile_join_kernel", st, dim3(kNumSMs, 16), 256, 0, [&](cudaLaunchConfig_t* cfg) {
+    cudaLaunchKernelEx(cfg, paged_attn_tile_join_kernel, a, w, D);
+  });
+}
+
+int launch_tiles(const PagedDev& c, const BatchDev& b, const AttnArgs& a, void* ws, cudaStream_t st) {
+  TileWs w;
+  carve_tile(ws, a.share, b.tokens, b.n, &w);
+  return c.D == 256 ? launch_tiles_d<256>(c, b, a, w, st) : launch_tiles_d<512>(c, b, a, w, st);
+}
+
+}  // namespace pa
+}  // namespace fmoe
