@@ -19,7 +19,7 @@
 // the one in use by 2^8.
 //
 // Warps: 0 copies (TMA, 16..64 rows of 64 dims a box, a box in one page),
-// 1 issues the products, 4..7 softmax, output and Q.
+// 1 issues the products, 4..11 softmax, output and Q.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -31,6 +31,7 @@ namespace pa {
 
 constexpr int kTile = 64;     // keys of a tile
 constexpr int kTileBegin = 2; // an item's beginning and end, in tiles of its time
+constexpr int kTileThreads = 384;
 constexpr int kUnit = 32768;  // bytes of a ring unit: 64 keys x 256 dims
 
 template <int D_>
@@ -40,7 +41,7 @@ struct Tile {
   static constexpr int OFF_Q = NU * kUnit;  // dims 256.. of Q, 4 blocks of [128 rows][128 bytes], swizzled
   static constexpr int OFF_BAR = OFF_Q + (D == 512 ? 65536 : 0);
   static constexpr int SMEM = OFF_BAR + 256 + 1024;
-  static_assert(SMEM <= 227 * 1024 - 256, "shared memory");
+  static_assert(SMEM <= 227 * 1024 - 1700, "shared memory");
 };
 
 // A tile of rows: what every kv head (and half) does with it.
@@ -98,11 +99,36 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, u
       "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)
       : "memory");
 }
-// V as B, rows of keys with the dims together (MN-major): 64-dim blocks of
-// [64 keys][128 bytes] 8 KB apart (leading offset), 8-key groups 1 KB apart.
-__device__ __forceinline__ uint64_t v_desc(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-         (2ull << 61);
+// Shared-memory descriptors in halves, so that a step along K is one addition:
+// 128-byte swizzle, 8-row groups 1 KB apart; K (K-major) has no leading offset
+// (1), V (MN-major: rows of keys with the dims together) 64-dim blocks of [64
+// keys][128 bytes] 8 KB apart.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t leading) { return ((addr >> 4) & 0x3FFF) | (leading << 16); }
+__device__ __forceinline__ uint64_t desc64(uint32_t lo) {
+  return (uint64_t)lo | ((uint64_t)(64u | (1u << 14) | (2u << 29)) << 32);
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
+}
+// Barrier of the softmax's 256 threads, true if `p` is in any of them.
+__device__ __forceinline__ bool softmax_any(bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred a, b;\n setp.ne.u32 a, %1, 0;\n barrier.cta.red.or.pred b, 1, 256, a;\n selp.u32 %0, 1, 0, b;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)p)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};\n" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 constexpr uint32_t kBMajorMN = 1u << 16;
 
@@ -228,13 +254,14 @@ struct Walk {
 };
 
 template <int D>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(kTileThreads, 1)
     paged_attn_tile_kernel(const __grid_constant__ CUtensorMap map, const PagedDev c, const AttnArgs a, const TileWs ws) {
   using C = Tile<D>;
   constexpr int NU = C::NU, KU = C::KU;
   extern __shared__ uint8_t sm_raw[];
   __shared__ uint32_t tmem_sh;
   __shared__ int failed_sh;
+  __shared__ float best_sh[2][128], sum_sh[128];
   uint8_t* sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
   uint64_t* empty = full + NU;
@@ -253,11 +280,11 @@ __global__ void __launch_bounds__(256, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i], 8);
       mbar_init(&pv_done[i], 1);
     }
-    mbar_init(q_full, 4);
-    mbar_init(o_free, 4);
+    mbar_init(q_full, 8);
+    mbar_init(o_free, 8);
     failed_sh = 0;
     mbar_fence_init();
   }
@@ -282,12 +309,12 @@ __global__ void __launch_bounds__(256, 1)
   w.u = u0;
   w.u1 = min(line, u0 + part);
   const bool any = u0 < w.u1;
-  if (any) {  // the row tile that the stretch begins in: a 256-way search
+  if (any) {  // the row tile that the stretch begins in: a 384-way search
     w.hh = (int)(u0 / w.total);
     const int64_t r = u0 - w.hh * w.total;
     int64_t lo = 0, n = w.count;
     while (n > 1) {
-      const int64_t step = (n + 255) / 256, k = lo + tid * step;
+      const int64_t step = (n + kTileThreads - 1) / kTileThreads, k = lo + tid * step;
       const int hits = __syncthreads_count(tid * step < n && __ldcg(reinterpret_cast<const long long*>(&ws.list[min(k, w.count - 1)].before)) <= r);
       lo += (hits - 1) * step;
       n = min(step, w.count - lo);
@@ -342,89 +369,99 @@ __global__ void __launch_bounds__(256, 1)
     // every copy issued lands before the CTA ends
     for (int k = max(0, n - NU); k < n; ++k) tc::drain_wait(&full[k % NU], (k / NU) & 1);
   } else if (any && warp == 1) {
-    // ---- products
-    if (lane == 0) {
-      const uint32_t id_s = tc::idesc_n(kTile), id_o = tc::idesc_n(256) | kBMajorMN;
-      int n = 0, g = 0, item = 0;  // units, tiles, items so far
-      while (w.load(ws)) {
-        auto scores = [&](int j) {  // S_j of the item's tile j (j-th here)
-          const uint32_t d = tS + ((g + j) & 1) * kTile;
+    // ---- products: the whole warp walks and waits, so that what an instruction
+    // takes stays in uniform registers; one lane issues
+    const bool lead = elect_one();
+    const uint32_t id_s = tc::idesc_n(kTile), id_o = tc::idesc_n(256) | kBMajorMN;
+    const uint32_t ring = smem_u32(sm), kd = desc_lo(ring, 1), vd = desc_lo(ring, 8192 >> 4);
+    int n = 0, s = 0, ph = 0, g = 0, item = 0;  // units, their slot and phase; tiles, items so far
+    auto step = [&]() {
+      ++n;
+      if (++s == NU) {
+        s = 0;
+        ph ^= 1;
+      }
+    };
+    while (w.load(ws)) {
+      const int tiles = __shfl_sync(0xffffffffu, w.k1 - w.k0, 0);
+      auto scores = [&](int gj) {  // S of tile gj
+        const uint32_t d = tS + (gj & 1) * kTile;
 #pragma unroll
-          for (int u = 0; u < KU; ++u, ++n) {
-            const int s = n % NU;
-            tc::pwait(&full[s], (n / NU) & 1, failed, ws.status, 602);
-            tc::tc_fence_after();
-            const uint32_t kb = smem_u32(sm + s * kUnit);
+        for (int u = 0; u < KU; ++u) {
+          tc::pwait(&full[s], ph, failed, ws.status, 602);
+          tc::tc_fence_after();
+          const uint32_t b = kd + s * (kUnit >> 4);
+          if (lead) {
+            if (u == 0) {
 #pragma unroll
-            for (int ks = 0; ks < 16; ++ks) {
-              const uint64_t bd = tc::sw128_desc(kb + (ks >> 2) * 8192 + (ks & 3) * 32);
-              if (u == 0)
-                mma_ts(d, tQ + 8 * ks, bd, id_s, ks > 0);
-              else
-                tc::mma_ss(d, tc::sw128_desc(smem_u32(sm + C::OFF_Q) + (ks >> 2) * 16384 + (ks & 3) * 32), bd, id_s, 1);
+              for (int ks = 0; ks < 16; ++ks)
+                mma_ts(d, tQ + 8 * ks, desc64(b + (ks >> 2) * 512 + (ks & 3) * 2), id_s, ks > 0);
+            } else {
+              const uint32_t q = desc_lo(ring + C::OFF_Q, 1);
+#pragma unroll
+              for (int ks = 0; ks < 16; ++ks)
+                tc::mma_ss(d, desc64(q + (ks >> 2) * 1024 + (ks & 3) * 2), desc64(b + (ks >> 2) * 512 + (ks & 3) * 2), id_s, 1);
             }
             tc::mma_commit(&empty[s]);
           }
-          tc::mma_commit(&s_full[(g + j) & 1]);
-        };
-        const int tiles = w.k1 - w.k0;
-        tc::pwait(q_full, item & 1, failed, ws.status, 603);
-        tc::tc_fence_after();
-        scores(0);
-#pragma unroll 1
-        for (int j = 0; j < tiles; ++j) {
-          if (j + 1 < tiles) scores(j + 1);
-          tc::pwait(&p_full[(g + j) & 1], ((g + j) >> 1) & 1, failed, ws.status, 604);
-          if (j == 0 && item > 0) tc::pwait(o_free, (item - 1) & 1, failed, ws.status, 605);
-          const int s = n % NU;
-          tc::pwait(&full[s], (n / NU) & 1, failed, ws.status, 606);
-          tc::tc_fence_after();
-          const uint32_t vb = smem_u32(sm + s * kUnit), p = tS + ((g + j) & 1) * kTile;
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) mma_ts(tO, p + 8 * kk, v_desc(vb + kk * 2048), id_o, j > 0 || kk > 0);
-          tc::mma_commit(&empty[s]);
-          tc::mma_commit(&pv_done[(g + j) & 1]);
-          ++n;
-          if (*failed) break;
+          __syncwarp();
+          step();
         }
-        g += tiles;
-        ++item;
-        w.next();
-        if (*failed) break;
-      }
-      // the products in flight end before the CTA does (a failure may have left some barrier short)
-      if (g > 0) tc::drain_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
-    }
-  } else if (any && warp >= 4) {
-    // ---- softmax: a thread is a row
-    const int qw = warp & 3, row = qw * 32 + lane;
-    const uint32_t lane_at = (uint32_t)(qw * 32) << 16;
-    int g = 0, item = 0, units = 0;
-    int tok, col;  // the row's token of the tile, its head of the group
-    tok = row / a.share;
-    col = row - tok * a.share;
-    auto load_q = [&]() {  // this row of Q: dims 0 .. 255 to tensor memory, the others to shared memory
-      const int h = w.hh % c.Hkv;
-      const bool has = tok < w.r.tokens;
-      const bf16* q = a.q + (int64_t)(w.r.row0 + tok) * a.qs + (int64_t)(h * a.share + col) * D;
+        if (lead) tc::mma_commit(&s_full[gj & 1]);
+        __syncwarp();
+      };
+      tc::pwait(q_full, item & 1, failed, ws.status, 603);
+      tc::tc_fence_after();
+      scores(g);
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {  // 64 dims
+      for (int j = 0; j < tiles; ++j, ++g) {
+        if (j + 1 < tiles) scores(g + 1);
+        tc::pwait(&p_full[g & 1], (g >> 1) & 1, failed, ws.status, 604);
+        if (j == 0 && item > 0) tc::pwait(o_free, (item - 1) & 1, failed, ws.status, 605);
+        tc::pwait(&full[s], ph, failed, ws.status, 606);
+        tc::tc_fence_after();
+        if (lead) {
+          const uint32_t b = vd + s * (kUnit >> 4), p = tS + (g & 1) * kTile;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) mma_ts(tO, p + 8 * kk, desc64(b + kk * 128), id_o, j > 0 || kk > 0);
+          tc::mma_commit(&empty[s]);
+          tc::mma_commit(&pv_done[g & 1]);
+        }
+        __syncwarp();
+        step();
+      }
+      ++item;
+      w.next();
+      if (__any_sync(0xffffffffu, *failed)) break;
+    }
+    // the products in flight end before the CTA does (a failure may have left some barrier short)
+    if (g > 0) tc::drain_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
+  } else if (any && warp >= 4) {
+    // ---- softmax: two threads to a row, each half of a tile's keys, of Q's and of O's dims
+    const int qw = warp & 3, row = qw * 32 + lane, side = (warp - 4) >> 2;
+    const uint32_t lane_at = (uint32_t)(qw * 32) << 16;
+    const int tok = row / a.share, col = row - tok * a.share;  // the row's token of the tile, its head of the group
+    int g = 0, units = 0;
+    uint4 q[16];
+    auto fetch_q = [&](int d0) {  // 128 dims of this row of Q, all loads on their way together
+      const bool has = tok < w.r.tokens;
+      const bf16* p = a.q + (int64_t)(w.r.row0 + tok) * a.qs + (int64_t)(w.hh % c.Hkv * a.share + col) * D + d0 + 128 * side;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) q[e] = has ? ldg_u4(p + 8 * e) : make_uint4(0, 0, 0, 0);
+    };
+    auto store_q = [&]() {  // to tensor memory, dims past 256 to shared memory
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
         uint32_t r[32];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint4 v = has ? ldg_u4(q + 64 * i + 8 * e) : make_uint4(0, 0, 0, 0);
-          r[4 * e] = v.x, r[4 * e + 1] = v.y, r[4 * e + 2] = v.z, r[4 * e + 3] = v.w;
-        }
-        tmem_st32(tQ + lane_at + 32 * i, r);
+        for (int e = 0; e < 8; ++e) r[4 * e] = q[8 * i + e].x, r[4 * e + 1] = q[8 * i + e].y, r[4 * e + 2] = q[8 * i + e].z, r[4 * e + 3] = q[8 * i + e].w;
+        tmem_st32(tQ + lane_at + 64 * side + 32 * i, r);
       }
       if constexpr (D == 512) {
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i)
+        fetch_q(256);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint4 v = has ? ldg_u4(q + 256 + 64 * i + 8 * e) : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(sm + C::OFF_Q + i * 16384 + row * 128 + ((e ^ (row & 7)) << 4)) = v;
-          }
+        for (int e = 0; e < 16; ++e)
+          *reinterpret_cast<uint4*>(sm + C::OFF_Q + (2 * side + (e >> 3)) * 16384 + row * 128 + (((e ^ row) & 7) << 4)) = q[e];
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       }
       tmem_st_wait();
@@ -433,16 +470,19 @@ __global__ void __launch_bounds__(256, 1)
       if (lane == 0) mbar_arrive(q_full);
     };
     bool more = w.load(ws);
-    if (more) load_q();
+    if (more) {
+      fetch_q(0);
+      store_q();
+    }
     while (more) {
       const RowTile r = w.r;
       const int k0 = w.k0, k1 = w.k1, h = w.hh % c.Hkv, half = w.hh / c.Hkv, tiles = k1 - k0;
       const int64_t s0 = w.s0;
       const int p = r.p0 + min(tok, r.tokens - 1), pl = r.p0 + r.tokens - 1;  // the row's position, the last row's
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f;  // l: of this side's keys
       int entry = -1, entry0 = -64;  // lanes hold the pages of 8 tiles' 16-key granules
 #pragma unroll 1
-      for (int j = 0; j < tiles; ++j) {
+      for (int j = 0; j < tiles; ++j, ++g) {
         const int k = k0 + j, j0 = kTile * (k < r.ns ? k : r.low_tile + k - r.ns);
         if (k >= entry0 + 8) {
           entry0 = k;
@@ -451,103 +491,113 @@ __global__ void __launch_bounds__(256, 1)
         }
         const uint32_t here = (__ballot_sync(0xffffffffu, entry >= 0) >> (4 * (k - entry0))) & 15;
         const bool whole = here == 15 && j0 + kTile - 1 <= r.p0 && (!a.window || j0 > pl - a.window || j0 + kTile - 1 < a.sinks);
-        const uint32_t tSj = tS + lane_at + ((g + j) & 1) * kTile;
-        tc::pwait(&s_full[(g + j) & 1], ((g + j) >> 1) & 1, failed, ws.status, 607);
+        const uint32_t tSj = tS + lane_at + (g & 1) * kTile;
+        tc::pwait(&s_full[g & 1], (g >> 1) & 1, failed, ws.status, 607);
         tc::tc_fence_after();
-        float s[2][32];
-        tmem_ld32(tSj, s[0]);
-        tmem_ld32(tSj + 32, s[1]);
+        float s[32];
+        tmem_ld32(tSj + 32 * side, s);
         tc::tmem_ld_wait();
         // the scale is part of the exponent's fma, except where scores are masked
         // (or it is not positive, and a maximum would not pass through it)
         float mul = a.sl;
         if (!whole || !(a.sl > 0.f)) {
           mul = 1.f;
+          const int jb = j0 + 32 * side;
+          const uint32_t hb = here >> (2 * side);
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            const int jj = j0 + i;
-            const bool see = ((here >> (i >> 4)) & 1) && jj <= p && (!a.window || jj > p - a.window || jj < a.sinks);
-            s[i >> 5][i & 31] = see ? s[i >> 5][i & 31] * a.sl : -INFINITY;
+          for (int i = 0; i < 32; ++i) {
+            const int jj = jb + i;
+            const bool see = ((hb >> (i >> 4)) & 1) && jj <= p && (!a.window || jj > p - a.window || jj < a.sinks);
+            s[i] = see ? s[i] * a.sl : -INFINITY;
           }
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i >> 5][i & 31]);
-        const float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
-        if (__any_sync(0xffffffffu, best > m + 8.f)) {
+        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+        float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+        // (the barrier also has every thread's scores read before any weight is written over them)
+        if (softmax_any(best > m + 8.f)) {
+          best_sh[side][row] = best;
+          softmax_any(false);
+          best = fmaxf(best, best_sh[side ^ 1][row]);
           const float mn = fmaxf(m, best), f = m == mn ? 1.f : ex2(m - mn);
           m = mn;
           l *= f;
           if (j > 0) {
-            tc::pwait(&pv_done[(g + j - 1) & 1], ((g + j - 1) >> 1) & 1, failed, ws.status, 608);
+            tc::pwait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, failed, ws.status, 608);
             tc::tc_fence_after();
+            if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-              float o[32];
-              uint32_t u[32];
-              tmem_ld32(tO + lane_at + 32 * i, o);
-              tc::tmem_ld_wait();
+              for (int i = 0; i < 4; ++i) {
+                float o[32];
+                uint32_t u[32];
+                tmem_ld32(tO + lane_at + 128 * side + 32 * i, o);
+                tc::tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(o[e] * f);
-              tmem_st32(tO + lane_at + 32 * i, u);
+                for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(o[e] * f);
+                tmem_st32(tO + lane_at + 128 * side + 32 * i, u);
+              }
             }
           }
         }
-        const float ref = m == -INFINITY ? 0.f : m;
-        uint32_t pk[32];
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float ref = m == -INFINITY ? 0.f : -m;
+        uint32_t pk[16];
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float x = s[i >> 4][(2 * i) & 31], y = s[i >> 4][(2 * i + 1) & 31];
-          x = ex2(fmaf(x, mul, -ref));
-          y = ex2(fmaf(y, mul, -ref));
-          sum[i & 3] += x + y;
+        for (int i = 0; i < 16; ++i) {
+          const float x = ex2(fmaf(s[2 * i], mul, ref)), y = ex2(fmaf(s[2 * i + 1], mul, ref));
+          sum[0] += x;
+          sum[1] += y;
           pk[i] = pack_bf16x2(x, y);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st32(tSj, pk);
+        l += sum[0] + sum[1];
+        tmem_st16(tSj + 16 * side, pk);
         // Rows of V that no row of the tile sees can hold anything: zeros instead
         const bool seen = whole || (here == 15 && j0 + kTile - 1 < r.hi && (j0 >= r.low || j0 + kTile - 1 < a.sinks));
         if (!seen) {
-          const int n = units + KU * min(j + 2, tiles) + j, sv = n % NU;  // V_j's unit
+          const int n = units + KU * min(j + 2, tiles) + j, sv = n % NU;  // this tile's unit of V
           tc::pwait(&full[sv], (n / NU) & 1, failed, ws.status, 609);
-          uint8_t* vb = sm + sv * kUnit;
-          const int t4 = tid & 127;  // a key per pair of threads, 2 of the 4 blocks each
-          const int jj = j0 + (t4 >> 1);
-          if (!(((here >> (t4 >> 5)) & 1) && jj < r.hi && (jj >= r.low || jj < a.sinks))) {
+          const int t4 = tid - 128, key = t4 >> 2, jj = j0 + key;  // four threads to a key, a block of 64 dims each
+          if (!(((here >> (key >> 4)) & 1) && jj < r.hi && (jj >= r.low || jj < a.sinks))) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              *reinterpret_cast<uint4*>(vb + ((t4 & 1) * 2 + (e >> 3)) * 8192 + (t4 >> 1) * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<uint4*>(sm + sv * kUnit + (t4 & 3) * 8192 + key * 128 + e * 16) = make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         }
         tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[(g + j) & 1]);
-        if (__any_sync(0xffffffffu, *failed)) break;
+        if (lane == 0) mbar_arrive(&p_full[g & 1]);
       }
       units += (KU + 1) * tiles;
+      // the row's sum over both sides
+      if (side) sum_sh[row] = l;
+      softmax_any(false);
+      if (!side) l += sum_sh[row];
+      softmax_any(false);
+      if (!side) sum_sh[row] = l;
+      softmax_any(false);
+      l = sum_sh[row];
       // the next item's Q before this one's output: its first scores run meanwhile
-      tc::pwait(&pv_done[(g + tiles - 1) & 1], ((g + tiles - 1) >> 1) & 1, failed, ws.status, 610);
-      tc::tc_fence_after();
-      g += tiles;
-      w.next();
-      more = !*failed && w.load(ws);
-      more = __all_sync(0xffffffffu, more);
-      if (more) load_q();
       const int64_t e0 = s0, e1 = s0 + r.tiles;  // the item on the line
+      w.next();
+      more = !softmax_any(*failed) && w.load(ws);
+      if (more) fetch_q(0);
+      tc::pwait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, failed, ws.status, 610);
+      tc::tc_fence_after();
+      if (more) store_q();
       const int cf = e0 >= u0 ? (int)blockIdx.x : (int)(e0 / part), cl = e1 <= w.u1 ? (int)blockIdx.x : (int)((e1 - 1) / part);
-      const bool has = tok < r.tokens && row < 128 / a.share * a.share;
+      const uint32_t tOs = tO + lane_at + 128 * side;
       if (cf == cl) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        bf16* o = a.out + ((int64_t)(r.row0 + tok) * a.Hq + h * a.share + col) * D + 256 * half;
+        bf16* o = a.out + ((int64_t)(r.row0 + tok) * a.Hq + h * a.share + col) * D + 256 * half + 128 * side;
 #pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           float v[32];
-          tmem_ld32(tO + lane_at + 32 * i, v);
+          tmem_ld32(tOs + 32 * i, v);
           tc::tmem_ld_wait();
-          if (has)
+          if (tok < r.tokens)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               *reinterpret_cast<uint4*>(o + 32 * i + 8 * e) =
@@ -556,18 +606,18 @@ __global__ void __launch_bounds__(256, 1)
         }
       } else {
         const int slot = 2 * blockIdx.x + (e0 > u0);
-        float* o = ws.o + ((int64_t)slot * 128 + row) * 256;
-        ws.ml[slot * 128 + row] = make_float2(m, l);
+        float* o = ws.o + ((int64_t)slot * 128 + row) * 256 + 128 * side;
+        if (side == 0) ws.ml[slot * 128 + row] = make_float2(m, l);
 #pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           float v[32];
-          tmem_ld32(tO + lane_at + 32 * i, v);
+          tmem_ld32(tOs + 32 * i, v);
           tc::tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             *reinterpret_cast<float4*>(o + 32 * i + 4 * e) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
         }
-        if (cf < (int)blockIdx.x && cl == (int)blockIdx.x && row == 0) {
+        if (cf < (int)blockIdx.x && cl == (int)blockIdx.x && row == 0 && side == 0) {
           TileSplit* t = ws.split + blockIdx.x;
           t->row0 = r.row0;
           t->rows = r.tokens * a.share;
@@ -580,7 +630,6 @@ __global__ void __launch_bounds__(256, 1)
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
-      ++item;
     }
   }
   tc::tc_fence_before();
@@ -676,7 +725,7 @@ static int launch_tiles_d(const PagedDev& c, const BatchDev& b, const AttnArgs& 
     paged_attn_plan_kernel<<<1, 1024, 0, st>>>(c, b, a, w);
   }
   if (int rc = check_launch("paged_attn_plan_kernel")) return rc;
-  if (int rc = launch_pdl("paged_attn_tile_kernel", st, dim3(kNumSMs), 256, Tile<D>::SMEM, [&](cudaLaunchConfig_t* cfg) {
+  if (int rc = launch_pdl("paged_attn_tile_kernel", st, dim3(kNumSMs), kTileThreads, Tile<D>::SMEM, [&](cudaLaunchConfig_t* cfg) {
         cudaLaunchKernelEx(cfg, paged_attn_tile_kernel<D>, map, c, a, w);
       }))
     return rc;
