@@ -18,8 +18,10 @@
 // ones); O is rescaled, by the softmax's warps, only when a row's maximum passes
 // the one in use by 2^8.
 //
-// Warps: 0 copies (TMA, 16..64 rows of 64 dims a box, a box in one page),
-// 1 issues the products, 4..11 softmax, output and Q.
+// Warps: 0 copies (TMA, 16..64 rows of 64 dims a box, a box in one page), 1
+// issues the products, 4..11 softmax (two threads to a row, half of a tile's keys
+// each), 12..15 the edges of items: Q in, output out, under the products of the
+// neighbouring items.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -31,7 +33,7 @@ namespace pa {
 
 constexpr int kTile = 64;     // keys of a tile
 constexpr int kTileBegin = 2; // an item's beginning and end, in tiles of its time
-constexpr int kTileThreads = 384;
+constexpr int kTileThreads = 512;
 constexpr int kUnit = 32768;  // bytes of a ring unit: 64 keys x 256 dims
 
 template <int D_>
@@ -40,8 +42,9 @@ struct Tile {
   static constexpr int NU = D == 256 ? 6 : 5;
   static constexpr int OFF_Q = NU * kUnit;  // dims 256.. of Q, 4 blocks of [128 rows][128 bytes], swizzled
   static constexpr int OFF_BAR = OFF_Q + (D == 512 ? 65536 : 0);
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;
-  static_assert(SMEM <= 227 * 1024 - 1700, "shared memory");
+  static constexpr int OFF_ML = OFF_BAR + 224;
+  static constexpr int SMEM = OFF_ML + 2560;  // the base is 1024-byte aligned, as the swizzle wants it
+  static_assert(SMEM <= 227 * 1024 - 32, "shared memory");
 };
 
 // A tile of rows: what every kv head (and half) does with it.
@@ -112,13 +115,20 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
   return p != 0;
 }
-// Barrier of the softmax's 256 threads, true if `p` is in any of them.
-__device__ __forceinline__ bool softmax_any(bool p) {
+// tc::pwait whose common case, a phase that is over, costs a poll.
+__device__ __noinline__ void wait_long(uint64_t* bar, uint32_t parity, volatile int* failed, int* status, int site) {
+  tc::pwait(bar, parity, failed, status, site);
+}
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* failed, int* status, int site) {
+  if (!tc::try_wait(bar, parity)) wait_long(bar, parity, failed, status, site);
+}
+// Barrier `id` of the two warps that share rows, true if `p` is in any thread.
+__device__ __forceinline__ bool pair_any(bool p, int id) {
   uint32_t r;
   asm volatile(
-      "{\n .reg .pred a, b;\n setp.ne.u32 a, %1, 0;\n barrier.cta.red.or.pred b, 1, 256, a;\n selp.u32 %0, 1, 0, b;\n}\n"
+      "{\n .reg .pred a, b;\n setp.ne.u32 a, %1, 0;\n barrier.cta.red.or.pred b, %2, 64, a;\n selp.u32 %0, 1, 0, b;\n}\n"
       : "=r"(r)
-      : "r"((uint32_t)p)
+      : "r"((uint32_t)p), "r"(id)
       : "memory");
   return r != 0;
 }
@@ -129,6 +139,21 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+// Stores of 32 bytes of a row.
+__device__ __forceinline__ void st_global32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// Keeps of 32 scores, times the scale, those whose bit is set.
+__device__ __forceinline__ void keep(float (&s)[32], uint32_t bits, float sl) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i] = bits & (1u << i) ? s[i] * sl : -INFINITY;
+}
+// Bits of the positions jb .. jb + 31 that lie below `end`.
+__device__ __forceinline__ uint32_t below(int jb, int end) {
+  return end <= jb ? 0u : end - jb >= 32 ? ~0u : (1u << (end - jb)) - 1;
 }
 constexpr uint32_t kBMajorMN = 1u << 16;
 
@@ -258,11 +283,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     paged_attn_tile_kernel(const __grid_constant__ CUtensorMap map, const PagedDev c, const AttnArgs a, const TileWs ws) {
   using C = Tile<D>;
   constexpr int NU = C::NU, KU = C::KU;
-  extern __shared__ uint8_t sm_raw[];
-  __shared__ uint32_t tmem_sh;
-  __shared__ int failed_sh;
-  __shared__ float best_sh[2][128], sum_sh[128];
-  uint8_t* sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
+  extern __shared__ __align__(1024) uint8_t sm[];
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(sm + C::OFF_ML - 16);
+  int* failed_at = reinterpret_cast<int*>(tmem_at + 1);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
   uint64_t* empty = full + NU;
   uint64_t* s_full = empty + NU;    // [2]
@@ -270,7 +293,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* pv_done = p_full + 2;   // [2]: the scores of tile j are in after the product of tile j - 2
   uint64_t* q_full = pv_done + 2;
   uint64_t* o_free = q_full + 1;
-  volatile int* failed = &failed_sh;
+  uint64_t* qk_done = o_free + 1;   // the item's scores are all computed: Q can go
+  uint64_t* l_full = qk_done + 1;   // the item's weights are all there, its rows' maxima and sums with them
+  volatile int* failed = failed_at;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -283,13 +308,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&p_full[i], 8);
       mbar_init(&pv_done[i], 1);
     }
-    mbar_init(q_full, 8);
-    mbar_init(o_free, 8);
-    failed_sh = 0;
+    mbar_init(q_full, 4);
+    mbar_init(o_free, 4);
+    mbar_init(qk_done, 1);
+    mbar_init(l_full, 8);
+    *failed_at = 0;
     mbar_fence_init();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_sh)), "r"(512)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_at)), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
@@ -298,7 +325,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  const uint32_t tmem = tmem_sh, tO = tmem, tQ = tmem + 256, tS = tmem + 384;
+  float* l_sh = reinterpret_cast<float*>(sm + C::OFF_ML);  // [2 items][128] sums, zero between uses
+  float* m_sh = l_sh + 256;                                 // [2 items][128] maxima
+  float* x_sh = m_sh + 256;                                 // [128] between the two threads of a row
+  const uint32_t tmem = *tmem_at, tO = tmem, tQ = tmem + 256, tS = tmem + 384;
 
   Walk w;
   w.total = __ldcg(reinterpret_cast<const long long*>(ws.total));
@@ -309,7 +339,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   w.u = u0;
   w.u1 = min(line, u0 + part);
   const bool any = u0 < w.u1;
-  if (any) {  // the row tile that the stretch begins in: a 384-way search
+  if (any) {  // the row tile that the stretch begins in: a 512-way search
     w.hh = (int)(u0 / w.total);
     const int64_t r = u0 - w.hh * w.total;
     int64_t lo = 0, n = w.count;
@@ -323,6 +353,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     w.i = lo;
   }
   if (tid == 0) ws.split[blockIdx.x].rows = 0;
+  if (tid < 256) l_sh[tid] = 0.f;
   __syncthreads();
 
   if (any && warp == 0) {
@@ -334,7 +365,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       int entry = -1, entry0 = -64;  // lanes hold the pages of 32 boxes
       auto copy = [&](int k, int which, int xd) {  // unit of tile k: dims xd .. xd + 255
         const int s = n % NU;
-        if (n >= NU) tc::pwait(&empty[s], ((n / NU) - 1) & 1, failed, ws.status, 601);
+        if (n >= NU) wait(&empty[s], ((n / NU) - 1) & 1, failed, ws.status, 601);
         const int b0 = k * per;
         if (b0 < entry0 || b0 + per > entry0 + 32) {
           entry0 = b0;
@@ -388,7 +419,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t d = tS + (gj & 1) * kTile;
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
-          tc::pwait(&full[s], ph, failed, ws.status, 602);
+          wait(&full[s], ph, failed, ws.status, 602);
           tc::tc_fence_after();
           const uint32_t b = kd + s * (kUnit >> 4);
           if (lead) {
@@ -402,33 +433,38 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               for (int ks = 0; ks < 16; ++ks)
                 tc::mma_ss(d, desc64(q + (ks >> 2) * 1024 + (ks & 3) * 2), desc64(b + (ks >> 2) * 512 + (ks & 3) * 2), id_s, 1);
             }
+            if (u == KU - 1) tc::mma_commit(&s_full[gj & 1]);
             tc::mma_commit(&empty[s]);
           }
           __syncwarp();
           step();
         }
-        if (lead) tc::mma_commit(&s_full[gj & 1]);
-        __syncwarp();
       };
-      tc::pwait(q_full, item & 1, failed, ws.status, 603);
+      wait(q_full, item & 1, failed, ws.status, 603);
       tc::tc_fence_after();
       scores(g);
+      if (tiles > 1) scores(g + 1);
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j, ++g) {
-        if (j + 1 < tiles) scores(g + 1);
-        tc::pwait(&p_full[g & 1], (g >> 1) & 1, failed, ws.status, 604);
-        if (j == 0 && item > 0) tc::pwait(o_free, (item - 1) & 1, failed, ws.status, 605);
-        tc::pwait(&full[s], ph, failed, ws.status, 606);
+        if (j == max(tiles - 2, 0)) {
+          if (lead) tc::mma_commit(qk_done);
+          __syncwarp();
+        }
+        wait(&full[s], ph, failed, ws.status, 606);
+        if (j == 0 && item > 0) wait(o_free, (item - 1) & 1, failed, ws.status, 605);
+        wait(&p_full[g & 1], (g >> 1) & 1, failed, ws.status, 604);
         tc::tc_fence_after();
         if (lead) {
           const uint32_t b = vd + s * (kUnit >> 4), p = tS + (g & 1) * kTile;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) mma_ts(tO, p + 8 * kk, desc64(b + kk * 128), id_o, j > 0 || kk > 0);
-          tc::mma_commit(&empty[s]);
+          for (int kk = 0; kk < 4; ++kk)  // a side's weights lie over its own scores
+            mma_ts(tO, p + 8 * (kk & 1) + 32 * (kk >> 1), desc64(b + kk * 128), id_o, j > 0 || kk > 0);
           tc::mma_commit(&pv_done[g & 1]);
+          tc::mma_commit(&empty[s]);
         }
         __syncwarp();
         step();
+        if (j + 2 < tiles) scores(g + 2);
       }
       ++item;
       w.next();
@@ -436,48 +472,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     // the products in flight end before the CTA does (a failure may have left some barrier short)
     if (g > 0) tc::drain_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
-  } else if (any && warp >= 4) {
-    // ---- softmax: two threads to a row, each half of a tile's keys, of Q's and of O's dims
-    const int qw = warp & 3, row = qw * 32 + lane, side = (warp - 4) >> 2;
-    const uint32_t lane_at = (uint32_t)(qw * 32) << 16;
-    const int tok = row / a.share, col = row - tok * a.share;  // the row's token of the tile, its head of the group
-    int g = 0, units = 0;
-    uint4 q[16];
-    auto fetch_q = [&](int d0) {  // 128 dims of this row of Q, all loads on their way together
-      const bool has = tok < w.r.tokens;
-      const bf16* p = a.q + (int64_t)(w.r.row0 + tok) * a.qs + (int64_t)(w.hh % c.Hkv * a.share + col) * D + d0 + 128 * side;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) q[e] = has ? ldg_u4(p + 8 * e) : make_uint4(0, 0, 0, 0);
-    };
-    auto store_q = [&]() {  // to tensor memory, dims past 256 to shared memory
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t r[32];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r[4 * e] = q[8 * i + e].x, r[4 * e + 1] = q[8 * i + e].y, r[4 * e + 2] = q[8 * i + e].z, r[4 * e + 3] = q[8 * i + e].w;
-        tmem_st32(tQ + lane_at + 64 * side + 32 * i, r);
-      }
-      if constexpr (D == 512) {
-        fetch_q(256);
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          *reinterpret_cast<uint4*>(sm + C::OFF_Q + (2 * side + (e >> 3)) * 16384 + row * 128 + (((e ^ row) & 7) << 4)) = q[e];
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      }
-      tmem_st_wait();
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    };
-    bool more = w.load(ws);
-    if (more) {
-      fetch_q(0);
-      store_q();
-    }
-    while (more) {
-      const RowTile r = w.r;
-      const int k0 = w.k0, k1 = w.k1, h = w.hh % c.Hkv, half = w.hh / c.Hkv, tiles = k1 - k0;
-      const int64_t s0 = w.s0;
+  } else if (any && warp >= 4 && warp < 12) {
+    // ---- softmax
+    const int row = (warp & 3) * 32 + lane, side = (warp - 4) >> 2;
+    const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
+    const int tok = row / a.share;  // the row's token of the tile
+    int g = 0, units = 0, item = 0;
+    while (w.load(ws)) {
+      const RowTile& r = w.r;
+      const int k0 = w.k0, k1 = w.k1, tiles = k1 - k0;
       const int p = r.p0 + min(tok, r.tokens - 1), pl = r.p0 + r.tokens - 1;  // the row's position, the last row's
       float m = -INFINITY, l = 0.f;  // l: of this side's keys
       int entry = -1, entry0 = -64;  // lanes hold the pages of 8 tiles' 16-key granules
@@ -492,7 +495,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t here = (__ballot_sync(0xffffffffu, entry >= 0) >> (4 * (k - entry0))) & 15;
         const bool whole = here == 15 && j0 + kTile - 1 <= r.p0 && (!a.window || j0 > pl - a.window || j0 + kTile - 1 < a.sinks);
         const uint32_t tSj = tS + lane_at + (g & 1) * kTile;
-        tc::pwait(&s_full[g & 1], (g >> 1) & 1, failed, ws.status, 607);
+        wait(&s_full[g & 1], (g >> 1) & 1, failed, ws.status, 607);
         tc::tc_fence_after();
         float s[32];
         tmem_ld32(tSj + 32 * side, s);
@@ -503,40 +506,35 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (!whole || !(a.sl > 0.f)) {
           mul = 1.f;
           const int jb = j0 + 32 * side;
-          const uint32_t hb = here >> (2 * side);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int jj = jb + i;
-            const bool see = ((hb >> (i >> 4)) & 1) && jj <= p && (!a.window || jj > p - a.window || jj < a.sinks);
-            s[i] = see ? s[i] * a.sl : -INFINITY;
-          }
+          uint32_t bits = below(jb, p + 1);
+          if (a.window) bits &= ~below(jb, p - a.window + 1) | below(jb, a.sinks);
+          bits &= ((here >> (2 * side)) & 1 ? ~0u : 0xffff0000u) & ((here >> (2 * side)) & 2 ? ~0u : 0x0000ffffu);
+          keep(s, bits, a.sl);
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-        float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
-        // (the barrier also has every thread's scores read before any weight is written over them)
-        if (softmax_any(best > m + 8.f)) {
-          best_sh[side][row] = best;
-          softmax_any(false);
-          best = fmaxf(best, best_sh[side ^ 1][row]);
-          const float mn = fmaxf(m, best), f = m == mn ? 1.f : ex2(m - mn);
+        const float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+        if (pair_any(best > m + 8.f, 1 + (warp & 3))) {  // in either warp of these rows
+          if (side) x_sh[row] = best;
+          pair_any(false, 1 + (warp & 3));
+          if (!side) x_sh[row] = fmaxf(fmaxf(m, best), x_sh[row]);
+          pair_any(false, 1 + (warp & 3));
+          const float mn = x_sh[row], f = m == mn ? 1.f : ex2(m - mn);
           m = mn;
           l *= f;
           if (j > 0) {
-            tc::pwait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, failed, ws.status, 608);
+            wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, failed, ws.status, 608);
             tc::tc_fence_after();
-            if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll 1
-              for (int i = 0; i < 4; ++i) {
-                float o[32];
-                uint32_t u[32];
-                tmem_ld32(tO + lane_at + 128 * side + 32 * i, o);
-                tc::tmem_ld_wait();
+            for (int i = 0; i < 4; ++i) {
+              float v[32];
+              uint32_t u[32];
+              tmem_ld32(tO + lane_at + 128 * side + 32 * i, v);
+              tc::tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(o[e] * f);
-                tmem_st32(tO + lane_at + 128 * side + 32 * i, u);
-              }
+              for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(v[e] * f);
+              tmem_st32(tO + lane_at + 128 * side + 32 * i, u);
             }
           }
         }
@@ -551,12 +549,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           pk[i] = pack_bf16x2(x, y);
         }
         l += sum[0] + sum[1];
-        tmem_st16(tSj + 16 * side, pk);
+        tmem_st16(tSj + 32 * side, pk);
         // Rows of V that no row of the tile sees can hold anything: zeros instead
         const bool seen = whole || (here == 15 && j0 + kTile - 1 < r.hi && (j0 >= r.low || j0 + kTile - 1 < a.sinks));
         if (!seen) {
           const int n = units + KU * min(j + 2, tiles) + j, sv = n % NU;  // this tile's unit of V
-          tc::pwait(&full[sv], (n / NU) & 1, failed, ws.status, 609);
+          wait(&full[sv], (n / NU) & 1, failed, ws.status, 609);
           const int t4 = tid - 128, key = t4 >> 2, jj = j0 + key;  // four threads to a key, a block of 64 dims each
           if (!(((here >> (key >> 4)) & 1) && jj < r.hi && (jj >= r.low || jj < a.sinks))) {
 #pragma unroll
@@ -565,59 +563,125 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         }
+        if (j + 1 == tiles) {
+          atomicAdd(&l_sh[(item & 1) * 128 + row], l);  // two addends to zero: their order is the same sum
+          if (side == 0) m_sh[(item & 1) * 128 + row] = m;
+        }
         tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[g & 1]);
+        if (lane == 0) {
+          mbar_arrive(&p_full[g & 1]);
+          if (j + 1 == tiles) mbar_arrive(l_full);
+        }
       }
       units += (KU + 1) * tiles;
-      // the row's sum over both sides
-      if (side) sum_sh[row] = l;
-      softmax_any(false);
-      if (!side) l += sum_sh[row];
-      softmax_any(false);
-      if (!side) sum_sh[row] = l;
-      softmax_any(false);
-      l = sum_sh[row];
-      // the next item's Q before this one's output: its first scores run meanwhile
-      const int64_t e0 = s0, e1 = s0 + r.tiles;  // the item on the line
+      ++item;
       w.next();
-      more = !softmax_any(*failed) && w.load(ws);
-      if (more) fetch_q(0);
-      tc::pwait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, failed, ws.status, 610);
-      tc::tc_fence_after();
-      if (more) store_q();
+      if (__any_sync(0xffffffffu, *failed)) break;
+    }
+  } else if (any && warp >= 12) {
+    // ---- edges: a thread is a row
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
+    const int tok = row / a.share, col = row - tok * a.share;  // the row's token of the tile, its head of the group
+    int g = 0, item = 0;
+    uint4 q[16];
+    auto fetch_q = [&](int d0) {  // 128 dims of this row of Q, all loads on their way together
+      const bool has = tok < w.r.tokens;
+      const bf16* p = a.q + (int64_t)(w.r.row0 + tok) * a.qs + (int64_t)(w.hh % c.Hkv * a.share + col) * D + d0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) q[e] = has ? ldg_u4(p + 8 * e) : make_uint4(0, 0, 0, 0);
+    };
+    auto store_q = [&]() {  // fetched dims 0 .. 127 and the others: to tensor memory, past 256 to shared memory
+#pragma unroll 1
+      for (int d = 0; d < 256; d += 128) {
+        if (d) fetch_q(d);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t r[32];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            r[4 * e] = q[8 * i + e].x, r[4 * e + 1] = q[8 * i + e].y, r[4 * e + 2] = q[8 * i + e].z, r[4 * e + 3] = q[8 * i + e].w;
+          tmem_st32(tQ + lane_at + d / 2 + 32 * i, r);
+        }
+      }
+      if constexpr (D == 512) {
+#pragma unroll 1
+        for (int d = 0; d < 256; d += 128) {
+          fetch_q(256 + d);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            *reinterpret_cast<uint4*>(sm + C::OFF_Q + (d / 64 + (e >> 3)) * 16384 + row * 128 + (((e ^ row) & 7) << 4)) = q[e];
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      }
+      tmem_st_wait();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    };
+    bool more = w.load(ws);
+    if (more) {
+      fetch_q(0);
+      store_q();
+    }
+    while (more) {
+      const RowTile r = w.r;
+      const int h = w.hh % c.Hkv, half = w.hh / c.Hkv;
+      const int64_t e0 = w.s0, e1 = w.s0 + r.tiles;  // the item on the line
+      g += w.k1 - w.k0;
       const int cf = e0 >= u0 ? (int)blockIdx.x : (int)(e0 / part), cl = e1 <= w.u1 ? (int)blockIdx.x : (int)((e1 - 1) / part);
-      const uint32_t tOs = tO + lane_at + 128 * side;
+      // the next item's Q as soon as this one's scores are computed
+      w.next();
+      more = __all_sync(0xffffffffu, !*failed) && w.load(ws);
+      if (more) {
+        fetch_q(0);
+        wait(qk_done, item & 1, failed, ws.status, 611);
+        tc::tc_fence_after();
+        store_q();
+      }
+      wait(l_full, item & 1, failed, ws.status, 612);
+      wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, failed, ws.status, 610);
+      tc::tc_fence_after();
+      const float l = l_sh[(item & 1) * 128 + row], m = m_sh[(item & 1) * 128 + row];
+      l_sh[(item & 1) * 128 + row] = 0.f;  // for the item after the next, whose Q comes later
       if (cf == cl) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        bf16* o = a.out + ((int64_t)(r.row0 + tok) * a.Hq + h * a.share + col) * D + 256 * half + 128 * side;
+        bf16* o = a.out + ((int64_t)(r.row0 + tok) * a.Hq + h * a.share + col) * D + 256 * half;
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
-          float v[32];
-          tmem_ld32(tOs + 32 * i, v);
+          float v[2][32];
+          tmem_ld32(tO + lane_at + 64 * i, v[0]);
+          tmem_ld32(tO + lane_at + 64 * i + 32, v[1]);
           tc::tmem_ld_wait();
           if (tok < r.tokens)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<uint4*>(o + 32 * i + 8 * e) =
-                  make_uint4(pack_bf16x2(v[8 * e] * inv, v[8 * e + 1] * inv), pack_bf16x2(v[8 * e + 2] * inv, v[8 * e + 3] * inv),
-                             pack_bf16x2(v[8 * e + 4] * inv, v[8 * e + 5] * inv), pack_bf16x2(v[8 * e + 6] * inv, v[8 * e + 7] * inv));
+            for (int e = 0; e < 4; ++e) {
+              uint32_t u[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) u[x] = pack_bf16x2(v[e >> 1][16 * (e & 1) + 2 * x] * inv, v[e >> 1][16 * (e & 1) + 2 * x + 1] * inv);
+              st_global32(o + 64 * i + 16 * e, u);
+            }
         }
       } else {
         const int slot = 2 * blockIdx.x + (e0 > u0);
-        float* o = ws.o + ((int64_t)slot * 128 + row) * 256 + 128 * side;
-        if (side == 0) ws.ml[slot * 128 + row] = make_float2(m, l);
+        float* o = ws.o + ((int64_t)slot * 128 + row) * 256;
+        ws.ml[slot * 128 + row] = make_float2(m, l);
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
           float v[32];
-          tmem_ld32(tOs + 32 * i, v);
+          tmem_ld32(tO + lane_at + 32 * i, v);
           tc::tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<float4*>(o + 32 * i + 4 * e) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          for (int e = 0; e < 4; ++e) {
+            uint32_t u[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) u[x] = __float_as_uint(v[8 * e + x]);
+            st_global32(o + 32 * i + 8 * e, u);
+          }
         }
-        if (cf < (int)blockIdx.x && cl == (int)blockIdx.x && row == 0 && side == 0) {
+        if (cf < (int)blockIdx.x && cl == (int)blockIdx.x && row == 0) {
           TileSplit* t = ws.split + blockIdx.x;
           t->row0 = r.row0;
           t->rows = r.tokens * a.share;
@@ -630,6 +694,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_free);
+      ++item;
     }
   }
   tc::tc_fence_before();
