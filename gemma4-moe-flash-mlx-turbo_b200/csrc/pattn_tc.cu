@@ -132,19 +132,69 @@ __device__ __forceinline__ bool pair_any(bool p, int id) {
       : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};\n" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
+__device__ __forceinline__ int floor_div(int x, int y) { return (x >= 0 ? x : x - y + 1) / y; }
 // Stores of 32 bytes of a row.
 __device__ __forceinline__ void st_global32(void* p, const uint32_t (&v)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
                "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two floats as one operand of the packed fp32 instructions.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of two values at or below 8 on the multiply-add pipes, for a share of the
+// weights: the special function unit's 4 lanes a clock would take all of a
+// tile's time.  x = n + f with n whole and |f| <= 1/2, 2^f by its Taylor series
+// to the fourth power (off by 4e-5 at most; a weight is rounded to 2^-9), n into
+// the exponent.  Below 2^-126: zero, as a masked score's -infinity.
+__device__ __forceinline__ void ex2_fma(uint64_t v, float& x, float& y) {
+  float a, b;
+  unpack2(v, a, b);
+  const bool za = a < -126.f, zb = b < -126.f;
+  v = pack2(za ? 0.f : a, zb ? 0.f : b);
+  const float big = 12582912.f;  // 1.5 * 2^23: adding it rounds to a whole number, in the low bits
+  const uint64_t r = add2(v, pack2(big, big)), n = add2(r, pack2(-big, -big));
+  const uint64_t f = fma2(n, pack2(-1.f, -1.f), v);
+  uint64_t q = fma2(f, pack2(0.0096181291f, 0.0096181291f), pack2(0.0555041087f, 0.0555041087f));  // ln2^4 / 4!, ln2^3 / 3!
+  q = fma2(q, f, pack2(0.2402265070f, 0.2402265070f));                                             // ln2^2 / 2
+  q = fma2(q, f, pack2(0.6931471806f, 0.6931471806f));
+  q = fma2(q, f, pack2(1.f, 1.f));
+  float ra, rb;
+  unpack2(r, ra, rb);
+  // (a product, so that what is no number stays none)
+  q = mul2(q, pack2(__uint_as_float((__float_as_uint(ra) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(rb) << 23) + 0x3f800000u)));
+  unpack2(q, a, b);
+  x = za ? 0.f : a;
+  y = zb ? 0.f : b;
 }
 // Keeps of 32 scores, times the scale, those whose bit is set.
 __device__ __forceinline__ void keep(float (&s)[32], uint32_t bits, float sl) {
@@ -262,9 +312,9 @@ struct Walk {
         ++hh;
       }
       const int4* p = reinterpret_cast<const int4*>(ws.list + i);
-      reinterpret_cast<int4*>(&r)[0] = __ldcg(p);
-      reinterpret_cast<int4*>(&r)[1] = __ldcg(p + 1);
-      reinterpret_cast<int4*>(&r)[2] = __ldcg(p + 2);
+      reinterpret_cast<int4*>(&r)[0] = __ldg(p);  // the list is final when this kernel reads it
+      reinterpret_cast<int4*>(&r)[1] = __ldg(p + 1);
+      reinterpret_cast<int4*>(&r)[2] = __ldg(p + 2);
       s0 = hh * total + r.before + kTileBegin;
       k0 = (int)max(u - s0, (int64_t)0);
       k1 = (int)min(u1 - s0, (int64_t)r.tiles);
@@ -484,16 +534,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int p = r.p0 + min(tok, r.tokens - 1), pl = r.p0 + r.tokens - 1;  // the row's position, the last row's
       float m = -INFINITY, l = 0.f;  // l: of this side's keys
       int entry = -1, entry0 = -64;  // lanes hold the pages of 8 tiles' 16-key granules
+      // tiles [ka, kb) are seen whole by every row (those of the first positions are looked at one by one)
+      const int shift = r.low_tile - r.ns;
+      const int ka = a.window ? max(r.ns, floor_div(pl - a.window, kTile) + 1 - shift) : r.ns;
+      const int kb = floor_div(r.p0 + 1, kTile) - shift;
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j, ++g) {
-        const int k = k0 + j, j0 = kTile * (k < r.ns ? k : r.low_tile + k - r.ns);
+        const int k = k0 + j;
         if (k >= entry0 + 8) {
           entry0 = k;
           const int kt = k + (lane >> 2), tile = kt < r.ns ? kt : r.low_tile + kt - r.ns;
           entry = kt < k1 ? page_of(c, r.seq, ((int64_t)tile * kTile + 16 * (lane & 3)) >> c.log_ps) : -1;
         }
         const uint32_t here = (__ballot_sync(0xffffffffu, entry >= 0) >> (4 * (k - entry0))) & 15;
-        const bool whole = here == 15 && j0 + kTile - 1 <= r.p0 && (!a.window || j0 > pl - a.window || j0 + kTile - 1 < a.sinks);
+        const bool whole = here == 15 && k >= ka && k < kb;
+        const int j0 = kTile * (k < r.ns ? k : shift + k);
         const uint32_t tSj = tS + lane_at + (g & 1) * kTile;
         wait(&s_full[g & 1], (g >> 1) & 1, failed, ws.status, 607);
         tc::tc_fence_after();
@@ -511,10 +566,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           bits &= ((here >> (2 * side)) & 1 ? ~0u : 0xffff0000u) & ((here >> (2 * side)) & 2 ? ~0u : 0x0000ffffu);
           keep(s, bits, a.sl);
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-        const float best = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+        for (int i = 4; i < 28; i += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[i + e], s[i + 4 + e]);
+        const float best = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], max3(s[28], s[29], s[30])), s[31]) * mul;
         if (pair_any(best > m + 8.f, 1 + (warp & 3))) {  // in either warp of these rows
           if (side) x_sh[row] = best;
           pair_any(false, 1 + (warp & 3));
@@ -539,17 +596,32 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.f : -m;
-        uint32_t pk[16];
-        float sum[2] = {0.f, 0.f};
+        const uint64_t slope = pack2(mul, mul), shift2 = pack2(ref, ref);
+        uint64_t sum = pack2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = ex2(fmaf(s[2 * i], mul, ref)), y = ex2(fmaf(s[2 * i + 1], mul, ref));
-          sum[0] += x;
-          sum[1] += y;
-          pk[i] = pack_bf16x2(x, y);
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t pk[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint64_t e = fma2(pack2(s[16 * hf + 2 * i], s[16 * hf + 2 * i + 1]), slope, shift2);
+            float x, y;
+            if (i % 4 == 3) {
+              ex2_fma(e, x, y);
+            } else {
+              unpack2(e, x, y);
+              x = ex2(x);
+              y = ex2(y);
+            }
+            sum = add2(sum, pack2(x, y));
+            pk[i] = pack_bf16x2(x, y);
+          }
+          tmem_st8(tSj + 32 * side + 8 * hf, pk);
         }
-        l += sum[0] + sum[1];
-        tmem_st16(tSj + 32 * side, pk);
+        {
+          float x, y;
+          unpack2(sum, x, y);
+          l += x + y;
+        }
         // Rows of V that no row of the tile sees can hold anything: zeros instead
         const bool seen = whole || (here == 15 && j0 + kTile - 1 < r.hi && (j0 >= r.low || j0 + kTile - 1 < a.sinks));
         if (!seen) {
