@@ -7,7 +7,7 @@
 // Two kernels share the rows of a step:
 //   paged_attn_split_kernel  sequences with at most 8 (row, head) pairs to a kv
 //                            head: decodes.  Bound by the pages' bytes.
-//   paged_attn_rows_kernel   the others, a CTA per (row, head).
+//   paged_attn_tile_kernel   the others (pattn_tc.cu).  Bound by the tensor cores.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -863,83 +863,6 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(const AttnArgs a, 
   store_tile<C>(r, f >> 5, v, L[0] == 0.f ? 0.f : 1.f / L[0], L[1] == 0.f ? 0.f : 1.f / L[1], lane);
 }
 
-// Lane l's values l * P .. of row `slot` of a block.
-template <int P>
-__device__ __forceinline__ void load_page_row(const PagedDev& c, const uint8_t* blk, int slot, int lane, float (&v)[P]) {
-  constexpr int D = 32 * P, LG = 64 / P, NG = P / 2;
-  if (c.bits == 16) {
-    const bf16* r = reinterpret_cast<const bf16*>(blk) + (int64_t)slot * D + lane * P;
-#pragma unroll
-    for (int i = 0; i < P; ++i) v[i] = bf2f(r[i]);
-    return;
-  }
-  const uint32_t* words = reinterpret_cast<const uint32_t*>(blk + slot * (D / 2));
-  const uint32_t pair = reinterpret_cast<const uint32_t*>(blk + c.ps * (D / 2) + slot * (D / 16))[lane / LG];
-  const float s = bf16lo(pair), b = bf16hi(pair);
-#pragma unroll
-  for (int o = 0; o < P / 8; ++o) {
-    const uint32_t w = words[((lane % LG) * (P / 8) + o) * NG + lane / LG];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[8 * o + i] = fmaf(s, (float)((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u), b);
-  }
-}
-
-// One CTA per (row, query head); a warp takes every 8th visible position.
-template <int P>
-__global__ void __launch_bounds__(256) paged_attn_rows_kernel(PagedDev c, BatchDev b, AttnArgs a) {
-  constexpr int D = 32 * P;
-  __shared__ float sm[8], sl[8], so[8][D];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t = blockIdx.x;
-  const int h = blockIdx.y, g = h / a.share;
-  int i = 0;
-  for (int k = 0; k < b.n; k += blockDim.x)
-    i += __syncthreads_count(k + (int)threadIdx.x < b.n && b.q_start[k + threadIdx.x + 1] <= t);
-  if (i >= b.n || (b.q_start[i + 1] - b.q_start[i]) * (int64_t)a.share <= kFewRows) return;
-  const int pos = b.kv_len[i] - b.q_start[i + 1] + (int)t;
-  const int low = a.window ? max(0, pos - a.window + 1) : 0;
-  const int first = a.window ? min(a.sinks, low) : 0;  // positions [0, first) and [low, pos]
-  float q[P], o[P], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < P; ++e) {
-    q[e] = bf2f(a.q[t * a.qs + (int64_t)h * D + lane * P + e]) * a.sl;
-    o[e] = 0.f;
-  }
-  const int end = min(pos + 1, c.max_blocks << c.log_ps);  // table rows hold no more
-  for (int n = warp; n < first + end - low; n += 8) {
-    const int j = n < first ? n : low + n - first;
-    const int page = page_of(c, b.seqs[i], j >> c.log_ps);
-    if (page < 0) continue;
-    float x[P], s = 0.f;
-    load_page_row<P>(c, page_block(c, a.layer, page, g, 0), j & (c.ps - 1), lane, x);
-#pragma unroll
-    for (int e = 0; e < P; ++e) s = fmaf(q[e], x[e], s);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    const float mn = fmaxf(m, s), f = ex2(m - mn), w = ex2(s - mn);
-    load_page_row<P>(c, page_block(c, a.layer, page, g, 1), j & (c.ps - 1), lane, x);
-    l = l * f + w;
-#pragma unroll
-    for (int e = 0; e < P; ++e) o[e] = o[e] * f + w * x[e];
-    m = mn;
-  }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int e = 0; e < P; ++e) so[warp][lane * P + e] = o[e];
-  __syncthreads();
-  float M = -INFINITY, L = 0.f;
-  for (int w = 0; w < 8; ++w) M = fmaxf(M, sm[w]);
-  for (int w = 0; w < 8; ++w) L += sm[w] > -INFINITY ? sl[w] * ex2(sm[w] - M) : 0.f;
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float x = 0.f;
-    for (int w = 0; w < 8; ++w) x += sm[w] > -INFINITY ? so[w][d] * ex2(sm[w] - M) : 0.f;
-    a.out[(t * a.Hq + h) * D + d] = __float2bfloat16_rn(L > 0.f ? x / L : 0.f);
-  }
-}
-
 // The scratch of a call: the status word, then what the parts of split items leave.
 size_t carve(void* base, const PagedDev& c, FewWs* w) {
   Carver k(base);
@@ -1051,14 +974,7 @@ int fmoe_paged_attend(const fmoe_paged_kv_t* cache, int layer, const void* q, in
   else
     rc = c.bits == 16 ? pa::launch_split<pa::Few<512, 16>>(c, b, a, w, st) : pa::launch_split<pa::Few<512, 4>>(c, b, a, w, st);
   if (rc || (int64_t)b.max_new * share <= pa::kFewRows) return rc;
-  if (c.bits == 16) return pa::launch_tiles(c, b, a, workspace, st);
-  ProfScope prof_("paged_attn_rows_kernel", st);
-  const dim3 grid((unsigned)b.tokens, (unsigned)q_heads);
-  if (c.D == 256)
-    pa::paged_attn_rows_kernel<8><<<grid, 256, 0, st>>>(c, b, a);
-  else
-    pa::paged_attn_rows_kernel<16><<<grid, 256, 0, st>>>(c, b, a);
-  return check_launch("paged_attn_rows_kernel");
+  return pa::launch_tiles(c, b, a, workspace, st);
 }
 
 }  // extern "C"

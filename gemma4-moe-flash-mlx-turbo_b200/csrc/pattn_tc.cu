@@ -22,6 +22,10 @@
 // issues the products, 4..11 softmax (two threads to a row, half of a tile's keys
 // each), 12..15 the edges of items: Q in, output out, under the products of the
 // neighbouring items.
+//
+// 4-bit pages: warp 0 copies codes and (scale, bias) pairs as they are, and six
+// more warps (2, 3, 16..19) turn them into the units that the bf16 copies would
+// have been: bf16(scale * code + bias), one rounding, 2^-9 of a value.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -33,16 +37,20 @@ namespace pa {
 
 constexpr int kTile = 64;     // keys of a tile
 constexpr int kTileBegin = 2; // an item's beginning and end, in tiles of its time
-constexpr int kTileThreads = 512;
+constexpr int kUnpackers = 6;  // warps that turn codes into units
 constexpr int kUnit = 32768;  // bytes of a ring unit: 64 keys x 256 dims
 
-template <int D_>
+template <int D_, int BITS_>
 struct Tile {
-  static constexpr int D = D_, HALVES = D / 256, KU = D / 256;  // KU: units of a K tile
-  static constexpr int NU = D == 256 ? 6 : 5;
+  static constexpr int D = D_, BITS = BITS_, HALVES = D / 256, KU = D / 256;  // KU: units of a K tile
+  static constexpr int THREADS = BITS == 16 ? 512 : 640;
+  static constexpr int NU = BITS == 16 ? (D == 256 ? 6 : 5) : (D == 256 ? 4 : 3);
+  // 4-bit: a stage is 64 rows of codes, then their pairs; a step 4 rows of it
+  static constexpr int CODES = 32 * D, STAGE = CODES + 4 * D, NS = BITS == 16 ? 0 : D == 256 ? 6 : 3, STEPS = kTile / 4;
   static constexpr int OFF_Q = NU * kUnit;  // dims 256.. of Q, 4 blocks of [128 rows][128 bytes], swizzled
-  static constexpr int OFF_BAR = OFF_Q + (D == 512 ? 65536 : 0);
-  static constexpr int OFF_ML = OFF_BAR + 224;
+  static constexpr int OFF_STAGE = OFF_Q + (D == 512 ? 65536 : 0);
+  static constexpr int OFF_BAR = OFF_STAGE + NS * STAGE;
+  static constexpr int OFF_ML = OFF_BAR + 304;
   static constexpr int SMEM = OFF_ML + 2560;  // the base is 1024-byte aligned, as the swizzle wants it
   static_assert(SMEM <= 227 * 1024 - 32, "shared memory");
 };
@@ -328,11 +336,25 @@ struct Walk {
   }
 };
 
-template <int D>
-__global__ void __launch_bounds__(kTileThreads, 1)
+// Eight 4-bit values as bf16: each code's bits go into the mantissa of 128, whose
+// subtraction is exact, and one fma rounds.
+__device__ __forceinline__ uint4 unpack8(uint32_t w, __nv_bfloat162 s, __nv_bfloat162 b) {
+  const uint32_t k = 0x43004300u;  // 128, 128
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t q = nib_pair(w, 4 * i);
+    const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q), *reinterpret_cast<const __nv_bfloat162*>(&k));
+    const __nv_bfloat162 v = __hfma2(c, s, b);
+    r[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 1)
     paged_attn_tile_kernel(const __grid_constant__ CUtensorMap map, const PagedDev c, const AttnArgs a, const TileWs ws) {
-  using C = Tile<D>;
-  constexpr int NU = C::NU, KU = C::KU;
+  constexpr int D = C::D, NU = C::NU, KU = C::KU, NS = C::NS;
   extern __shared__ __align__(1024) uint8_t sm[];
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(sm + C::OFF_ML - 16);
   int* failed_at = reinterpret_cast<int*>(tmem_at + 1);
@@ -345,13 +367,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* o_free = q_full + 1;
   uint64_t* qk_done = o_free + 1;   // the item's scores are all computed: Q can go
   uint64_t* l_full = qk_done + 1;   // the item's weights are all there, its rows' maxima and sums with them
+  uint64_t* st_full = l_full + 1;   // [NS] 4-bit: codes are there, and turned into units
+  uint64_t* st_empty = st_full + NS;
   volatile int* failed = failed_at;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     for (int i = 0; i < NU; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], C::BITS == 16 ? 1 : C::STEPS);
       mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&st_full[i], 1);
+      mbar_init(&st_empty[i], C::STEPS);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -389,12 +417,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   w.u = u0;
   w.u1 = min(line, u0 + part);
   const bool any = u0 < w.u1;
-  if (any) {  // the row tile that the stretch begins in: a 512-way search
+  if (any) {  // the row tile that the stretch begins in: a search by all threads at once
     w.hh = (int)(u0 / w.total);
     const int64_t r = u0 - w.hh * w.total;
     int64_t lo = 0, n = w.count;
     while (n > 1) {
-      const int64_t step = (n + kTileThreads - 1) / kTileThreads, k = lo + tid * step;
+      const int64_t step = (n + C::THREADS - 1) / C::THREADS, k = lo + tid * step;
       const int hits = __syncthreads_count(tid * step < n && __ldcg(reinterpret_cast<const long long*>(&ws.list[min(k, w.count - 1)].before)) <= r);
       lo += (hits - 1) * step;
       n = min(step, w.count - lo);
@@ -413,31 +441,47 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     while (w.load(ws)) {
       const int h = w.hh % c.Hkv, half = w.hh / c.Hkv;
       int entry = -1, entry0 = -64;  // lanes hold the pages of 32 boxes
-      auto copy = [&](int k, int which, int xd) {  // unit of tile k: dims xd .. xd + 255
-        const int s = n % NU;
-        if (n >= NU) wait(&empty[s], ((n / NU) - 1) & 1, failed, ws.status, 601);
-        const int b0 = k * per;
+      auto page_of_box = [&](int b0, int gr) {  // box gr of the tile whose first box is b0
         if (b0 < entry0 || b0 + per > entry0 + 32) {
           entry0 = b0;
           const int j = b0 + lane, kt = j / per, tile = kt < w.r.ns ? kt : w.r.low_tile + kt - w.r.ns;
           entry = kt < w.k1 ? page_of(c, w.r.seq, ((int64_t)tile * kTile + (j % per) * box) >> c.log_ps) : -1;
         }
-        const int gr = min(lane >> 2, per - 1), cb = lane & 3;
-        const int page = __shfl_sync(0xffffffffu, entry, b0 + gr - entry0);
+        return __shfl_sync(0xffffffffu, entry, b0 + gr - entry0);
+      };
+      auto copy = [&](int k, int which, int xd) {  // bf16: unit of tile k, dims xd .. xd + 255; 4-bit: its stage
+        constexpr int N = C::BITS == 16 ? NU : NS;
+        uint64_t* there = C::BITS == 16 ? full : st_full;
+        const int s = n % N;
+        if (n >= N) wait(C::BITS == 16 ? &empty[s] : &st_empty[s], ((n / N) - 1) & 1, failed, ws.status, 601);
         const int tile = k < w.r.ns ? k : w.r.low_tile + k - w.r.ns;
-        const int slot = (tile * kTile + gr * box) & (c.ps - 1);
-        // a page that is missing is read past the end: zeros
-        const int y = page >= 0 ? ((page * c.Hkv + h) * 2 + which) * c.ps + slot : 2 * c.num_pages * c.Hkv * c.ps;
-        if (!__any_sync(0xffffffffu, *failed)) {
-          if (lane == 0) mbar_arrive_expect_tx(&full[s], kUnit);
+        const int gr = C::BITS == 16 ? min(lane >> 2, per - 1) : min(lane >> 1, per - 1);
+        const int page = page_of_box(k * per, gr), slot = (tile * kTile + gr * box) & (c.ps - 1);
+        if (__any_sync(0xffffffffu, *failed)) return;
+        if constexpr (C::BITS == 16) {
+          const int cb = lane & 3;
+          // a page that is missing is read past the end: zeros
+          const int y = page >= 0 ? ((page * c.Hkv + h) * 2 + which) * c.ps + slot : 2 * c.num_pages * c.Hkv * c.ps;
+          if (lane == 0) mbar_arrive_expect_tx(&there[s], kUnit);
           __syncwarp();
-          if (lane < 4 * per) tc::tma2d(sm + s * kUnit + cb * 8192 + gr * box * 128, &map, xd + 64 * cb, y, &full[s]);
-          ++n;
+          if (lane < 4 * per) tc::tma2d(sm + s * kUnit + cb * 8192 + gr * box * 128, &map, xd + 64 * cb, y, &there[s]);
+        } else {
+          uint8_t* st = sm + C::OFF_STAGE + s * C::STAGE;
+          const bool go = lane < 2 * per && page >= 0;  // what a missing page leaves here is masked, and cleared, later
+          const int boxes = __popc(__ballot_sync(0xffffffffu, go)) / 2;
+          if (lane == 0) mbar_arrive_expect_tx(&there[s], boxes * box * (D / 2 + D / 16));
+          __syncwarp();
+          if (go && (lane & 1) == 0)
+            tc::tma3d(st + gr * box * (D / 2), &map, 0, slot, (page * c.Hkv + h) * 2 + which, &there[s]);
+          else if (go)
+            bulk_g2s(st + C::CODES + gr * box * (D / 16),
+                     page_block(c, a.layer, page, h, which) + c.ps * (D / 2) + slot * (D / 16), box * (D / 16), &there[s]);
         }
+        ++n;
       };
       auto copy_k = [&](int k) {
 #pragma unroll
-        for (int d = 0; d < KU; ++d) copy(k, 0, 256 * d);
+        for (int d = 0; d < (C::BITS == 16 ? KU : 1); ++d) copy(k, 0, 256 * d);
       };
       copy_k(w.k0);
 #pragma unroll 1
@@ -448,7 +492,60 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       w.next();
     }
     // every copy issued lands before the CTA ends
-    for (int k = max(0, n - NU); k < n; ++k) tc::drain_wait(&full[k % NU], (k / NU) & 1);
+    constexpr int N = C::BITS == 16 ? NU : NS;
+    for (int k = max(0, n - N); k < n; ++k) tc::drain_wait(C::BITS == 16 ? &full[k % N] : &st_full[k % N], (k / N) & 1);
+  } else if (any && C::BITS == 4 && (warp == 2 || warp == 3 || warp >= 16)) {
+    // ---- 4-bit: stages to units, a step of 4 keys a warp at a time: 8 lanes a key, a lane an octet of its groups
+    if constexpr (C::BITS == 4) {
+      const int me = warp < 4 ? warp - 2 : warp - 14, key0 = lane >> 3, oct = lane & 7;
+      int n = 0, u = 0;  // stages, units
+      while (w.load(ws)) {
+        const int half = w.hh / c.Hkv, tiles = w.k1 - w.k0;
+        auto turn = [&](bool v) {
+          const int s = n % NS, units = v ? 1 : KU;
+          wait(&st_full[s], (n / NS) & 1, failed, ws.status, 613);
+#pragma unroll
+          for (int i = 0; i < KU; ++i)
+            if (i < units && u + i >= NU) wait(&empty[(u + i) % NU], (((u + i) / NU) - 1) & 1, failed, ws.status, 614);
+          const uint8_t* st = sm + C::OFF_STAGE + s * C::STAGE;
+#pragma unroll 1
+          for (int i = (me + kUnpackers - (n * C::STEPS) % kUnpackers) % kUnpackers; i < C::STEPS; i += kUnpackers) {
+            const int key = 4 * i + key0;
+#pragma unroll
+            for (int hf = 0; hf < KU; ++hf) {  // 256 dims
+              if (v && hf != half) continue;
+              const uint4 codes = lds_u4(st + key * (D / 2) + oct * (D / 16) + hf * 16);
+              const uint4 pairs = lds_u4(st + C::CODES + key * (D / 16) + hf * 16);
+              const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w}, pw[4] = {pairs.x, pairs.y, pairs.z, pairs.w};
+              uint8_t* unit = sm + ((u + (v ? 0 : hf)) % NU) * kUnit + key * 128 + (((oct ^ key) & 7) << 4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 p = *reinterpret_cast<const __nv_bfloat162*>(&pw[e]);
+                *reinterpret_cast<uint4*>(unit + e * 8192) = unpack8(cw[e], __low2bfloat162(p), __high2bfloat162(p));
+              }
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // generic writes -> tensor-core reads
+            __syncwarp();
+            if (lane == 0) {
+#pragma unroll
+              for (int hf = 0; hf < KU; ++hf)
+                if (hf < units) mbar_arrive(&full[(u + hf) % NU]);
+              mbar_arrive(&st_empty[s]);
+            }
+          }
+          ++n;
+          u += units;
+        };
+        turn(false);
+#pragma unroll 1
+        for (int j = 0; j < tiles; ++j) {
+          if (j + 1 < tiles) turn(false);
+          turn(true);
+        }
+        w.next();
+        if (__any_sync(0xffffffffu, *failed)) break;
+      }
+    }
   } else if (any && warp == 1) {
     // ---- products: the whole warp walks and waits, so that what an instruction
     // takes stays in uniform registers; one lane issues
@@ -652,7 +749,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       w.next();
       if (__any_sync(0xffffffffu, *failed)) break;
     }
-  } else if (any && warp >= 12) {
+  } else if (any && warp >= 12 && warp < 16) {
     // ---- edges: a thread is a row
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
@@ -841,30 +938,41 @@ static int launch_pdl(const char* name, cudaStream_t st, dim3 grid, int threads,
   return check_launch(name);
 }
 
-template <int D>
-static int launch_tiles_d(const PagedDev& c, const BatchDev& b, const AttnArgs& a, const TileWs& w, cudaStream_t st) {
+template <class C>
+static int launch_tiles_c(const PagedDev& c, const BatchDev& b, const AttnArgs& a, const TileWs& w, cudaStream_t st) {
+  constexpr int D = C::D;
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
   std::call_once(once, [] {
-    err = cudaFuncSetAttribute(paged_attn_tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<D>::SMEM);
+    err = cudaFuncSetAttribute(paged_attn_tile_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   });
   if (err != cudaSuccess)
     return set_error(FMOE_ERR_CUDA, "paged_attend: shared memory attribute: %s", cudaGetErrorString(err));
-  const int64_t rows = 2ll * c.num_pages * c.Hkv * c.ps;
+  const int64_t blocks = 2ll * c.num_pages * c.Hkv;
+  const void* base = c.pages + a.layer * c.layer;
+  const cuuint32_t rows = (cuuint32_t)std::min(c.ps, kTile);
   CUtensorMap map;
-  const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)D * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)std::min(c.ps, kTile)};
-  if (int rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c.pages + a.layer * c.layer, dims, strides, box,
-                      CU_TENSOR_MAP_SWIZZLE_128B, "pages"))
-    return rc;
+  int rc;
+  if (C::BITS == 16) {
+    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)(blocks * c.ps)}, strides[1] = {(cuuint64_t)D * 2};
+    const cuuint32_t box[2] = {64, rows};
+    rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, "pages");
+  } else {
+    const cuuint64_t dims[3] = {(cuuint64_t)D / 2, (cuuint64_t)c.ps, (cuuint64_t)blocks};
+    const cuuint64_t strides[2] = {(cuuint64_t)D / 2, (cuuint64_t)c.block};
+    const cuuint32_t box[3] = {(cuuint32_t)D / 2, rows, 1};
+    rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE, "pages");
+  }
+  if (rc) return rc;
   {
     ProfScope prof_("paged_attn_plan_kernel", st);
     paged_attn_plan_kernel<<<1, 1024, 0, st>>>(c, b, a, w);
   }
-  if (int rc = check_launch("paged_attn_plan_kernel")) return rc;
-  if (int rc = launch_pdl("paged_attn_tile_kernel", st, dim3(kNumSMs), kTileThreads, Tile<D>::SMEM, [&](cudaLaunchConfig_t* cfg) {
-        cudaLaunchKernelEx(cfg, paged_attn_tile_kernel<D>, map, c, a, w);
-      }))
+  if ((rc = check_launch("paged_attn_plan_kernel"))) return rc;
+  if ((rc = launch_pdl(C::BITS == 16 ? "paged_attn_tile_kernel<bf16>" : "paged_attn_tile_kernel<4-bit>", st, dim3(kNumSMs),
+                       C::THREADS, C::SMEM, [&](cudaLaunchConfig_t* cfg) {
+                         cudaLaunchKernelEx(cfg, paged_attn_tile_kernel<C>, map, c, a, w);
+                       })))
     return rc;
   return launch_pdl("paged_attn_tile_join_kernel", st, dim3(kNumSMs, 16), 256, 0, [&](cudaLaunchConfig_t* cfg) {
     cudaLaunchKernelEx(cfg, paged_attn_tile_join_kernel, a, w, D);
@@ -874,7 +982,9 @@ static int launch_tiles_d(const PagedDev& c, const BatchDev& b, const AttnArgs& 
 int launch_tiles(const PagedDev& c, const BatchDev& b, const AttnArgs& a, void* ws, cudaStream_t st) {
   TileWs w;
   carve_tile(ws, a.share, b.tokens, b.n, &w);
-  return c.D == 256 ? launch_tiles_d<256>(c, b, a, w, st) : launch_tiles_d<512>(c, b, a, w, st);
+  if (c.D == 256)
+    return c.bits == 16 ? launch_tiles_c<Tile<256, 16>>(c, b, a, w, st) : launch_tiles_c<Tile<256, 4>>(c, b, a, w, st);
+  return c.bits == 16 ? launch_tiles_c<Tile<512, 16>>(c, b, a, w, st) : launch_tiles_c<Tile<512, 4>>(c, b, a, w, st);
 }
 
 }  // namespace pa
