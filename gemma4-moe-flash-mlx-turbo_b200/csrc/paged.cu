@@ -338,12 +338,10 @@ __global__ void __launch_bounds__(256) paged_copy_kernel(PagedDev c, const int32
 // storing a step's rows
 
 // The sequence of row t (n: none): how many sequences end at or before it.
-__device__ __forceinline__ int seq_of_row(const BatchDev& b, int64_t t) {
+__device__ __forceinline__ int seq_of_row(const BatchDev& b, int64_t t, int lane) {
   int count = 0;
-  for (int i = 0; i < b.n; i += blockDim.x) {
-    const int k = i + threadIdx.x;
-    count += __syncthreads_count(k < b.n && __ldg(b.q_start + k + 1) <= t);
-  }
+  for (int k = 0; k < b.n; k += 32)
+    count += __popc(__ballot_sync(0xffffffffu, k + lane < b.n && __ldg(b.q_start + min(k + lane, b.n - 1) + 1) <= t));
   return count;
 }
 
@@ -401,75 +399,118 @@ struct RowsIn {
   const bf16 *q, *k, *v, *qn, *kn;
   int64_t qs, ks, vs;  // row strides, values
   int Hq, rope;
+  int heads, chunks;   // heads that a warp takes of a row, and how often that goes into it
   float eps;
   double l2t;  // log2(theta)
   bf16* q_out;
 };
 
-// One CTA per row of the step; a warp takes heads of it.  NORM: norms and
-// rotation (append_qkv); otherwise k and v as they are.
+// A warp takes `heads` of the q | k | v heads of one row of the step at a time,
+// a lane P neighbouring dims of each.  NORM: norms and rotation (append_qkv);
+// otherwise k and v as they are.  Bound by the rows' bytes: four rows are on
+// their way while one is worked on, and nothing waits for another warp.  The
+// rates of the rotation are computed once per CTA (a thread a rate), a row's
+// cosines and sines once per warp, in registers, for all its heads.
+constexpr int kRowWarps = 8;
 template <int P, bool NORM>
-__global__ void __launch_bounds__(256) paged_rows_kernel(PagedDev c, int layer, BatchDev b, RowsIn a) {
-  constexpr int D = 32 * P;
-  __shared__ float tcos[NORM ? D / 2 : 1], tsin[NORM ? D / 2 : 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t = blockIdx.x;
-  const int i = seq_of_row(b, t);
-  if (i >= b.n) return;
-  const int len = b.kv_len[i], pos = len - b.q_start[i + 1] + (int)t;
-  const int half = a.rope / 2;
+__global__ void __launch_bounds__(32 * kRowWarps) paged_rows_kernel(PagedDev c, int layer, BatchDev b, RowsIn a) {
+  constexpr int D = 32 * P, V = P / 8;
+  __shared__ double rate[NORM ? D / 2 : 1];  // turns per position
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = a.rope / 2;
   if (NORM) {
-    // angle in turns = pos * theta^(-2j / rope) / 2 pi, reduced in 64 bits: a
-    // position of 10^5 times a 32-bit rate is off by a hundredth of a radian
-    for (int j = threadIdx.x; j < half; j += blockDim.x) {
-      const double turns = pos * (exp2(-(double)(2 * j) / a.rope * a.l2t) * 0.15915494309189535);
-      sincospif(2.0f * (float)(turns - rint(turns)), &tsin[j], &tcos[j]);
-    }
+    for (int j = threadIdx.x; j < half; j += blockDim.x)
+      rate[j] = exp2(-(double)(2 * j) / a.rope * a.l2t) * 0.15915494309189535;
     __syncthreads();
   }
-  const int page = pos >= 0 && pos < len ? page_of(c, b.seqs[i], pos >> c.log_ps) : -1;
-  const int slot = pos & (c.ps - 1);
-  for (int hh = warp; hh < (NORM ? a.Hq : 0) + 2 * c.Hkv; hh += blockDim.x / 32) {
-    float x[P];
-    const int h = NORM ? hh - a.Hq : hh;
-    const bool is_v = h >= c.Hkv;
-    const bf16* src = h < 0 ? a.q + t * a.qs + (int64_t)hh * D
-                      : is_v && a.v ? a.v + t * a.vs + (int64_t)(h - c.Hkv) * D
-                                    : a.k + t * a.ks + (int64_t)(is_v ? h - c.Hkv : h) * D;
-    if (h >= 0 && page < 0) continue;
-    load_row_f32<P>(src, lane, x);
-    if (NORM) {
-      float ss = 0.f;
+  const int total = (NORM ? a.Hq : 0) + 2 * c.Hkv;
+  const int64_t work = b.tokens * a.chunks;
+  int64_t held = -1;  // the row whose angles the lane holds
+  float cs[NORM ? P : 1], sn[NORM ? P : 1];
+  for (int64_t wi = (int64_t)blockIdx.x * kRowWarps + warp; wi < work; wi += (int64_t)gridDim.x * kRowWarps) {
+    const int64_t t = wi / a.chunks;
+    const int h0 = (int)(wi - t * a.chunks) * a.heads, h1 = min(h0 + a.heads, total);
+    auto source = [&](int hh) {
+      const int h = NORM ? hh - a.Hq : hh;
+      const bool is_v = h >= c.Hkv;
+      return h < 0 ? a.q + t * a.qs + (int64_t)hh * D
+                   : (is_v && a.v ? a.v + t * a.vs + (int64_t)(h - c.Hkv) * D
+                                  : a.k + t * a.ks + (int64_t)(is_v ? h - c.Hkv : h) * D);
+    };
+    uint4 raw[4][V];
+    auto fetch = [&](int hh, uint4 (&r)[V]) {
+      const uint4* p = reinterpret_cast<const uint4*>(source(min(hh, h1 - 1)) + lane * P);
 #pragma unroll
-      for (int e = 0; e < P; ++e) ss = fmaf(x[e], x[e], ss);
+      for (int i = 0; i < V; ++i) r[i] = p[i];
+    };
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float r = rsqrtf(ss / (float)D + a.eps);
-      if (is_v) {
+    for (int u = 0; u < 4; ++u) fetch(h0 + u, raw[u]);
+    const int i = seq_of_row(b, t, lane);
+    if (i >= b.n) continue;
+    const int len = __ldg(b.kv_len + i), pos = len - __ldg(b.q_start + i + 1) + (int)t;
+    const int page = pos >= 0 && pos < len ? page_of(c, __ldg(b.seqs + i), pos >> c.log_ps) : -1;
+    const int slot = pos & (c.ps - 1);
+    if (NORM && held != t) {
+      held = t;
+      // turns reduced in 64 bits: a position of 10^5 times a 32-bit rate is off by
+      // a hundredth of a radian
 #pragma unroll
-        for (int e = 0; e < P; ++e) x[e] *= r;
-      } else {
-        float wv[P];
-        load_row_f32<P>(h < 0 ? a.qn : a.kn, lane, wv);
-#pragma unroll
-        for (int e = 0; e < P; ++e) x[e] *= r * wv[e];
-        const int ofs = half / P;
-#pragma unroll
-        for (int e = 0; e < P; ++e) {
-          const float up = __shfl_down_sync(0xffffffffu, x[e], ofs & 31);
-          const float dn = __shfl_up_sync(0xffffffffu, x[e], ofs & 31);
-          const int d = lane * P + e;
-          if (d < half)
-            x[e] = x[e] * tcos[d] - up * tsin[d];
-          else if (d < 2 * half)
-            x[e] = x[e] * tcos[d - half] + dn * tsin[d - half];
+      for (int e = 0; e < P; ++e) {
+        const int d = lane * P + e;
+        cs[e] = 1.f;
+        sn[e] = 0.f;
+        if (d < 2 * half) {
+          const double turns = pos * rate[d < half ? d : d - half];
+          sincospif(2.0f * (float)(turns - rint(turns)), &sn[e], &cs[e]);
+          if (d < half) sn[e] = -sn[e];  // x cos - up sin, or x cos + dn sin
         }
       }
     }
-    if (h < 0)
-      store_row_bf16<P>(a.q_out + (t * a.Hq + hh) * D, lane, x);
-    else
-      store_page_row<P>(c, layer, page, slot, is_v ? h - c.Hkv : h, is_v, x, lane);
+    for (int g0 = h0; g0 < h1; g0 += 4) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int hh = g0 + u, h = NORM ? hh - a.Hq : hh;
+        if (hh >= h1) break;
+        const bool is_v = h >= c.Hkv;
+        float x[P];
+#pragma unroll
+        for (int i8 = 0; i8 < V; ++i8) {
+          const uint4 w = raw[u][i8];
+          x[8 * i8] = bf16lo(w.x), x[8 * i8 + 1] = bf16hi(w.x), x[8 * i8 + 2] = bf16lo(w.y), x[8 * i8 + 3] = bf16hi(w.y);
+          x[8 * i8 + 4] = bf16lo(w.z), x[8 * i8 + 5] = bf16hi(w.z), x[8 * i8 + 6] = bf16lo(w.w), x[8 * i8 + 7] = bf16hi(w.w);
+        }
+        fetch(hh + 4, raw[u]);
+        if (NORM) {
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < P; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float r = rsqrtf(ss / (float)D + a.eps);
+          if (is_v) {
+#pragma unroll
+            for (int e = 0; e < P; ++e) x[e] *= r;
+          } else {
+            float wv[P];
+            load_row_f32<P>(h < 0 ? a.qn : a.kn, lane, wv);
+            const int ofs = half / P;  // lanes between the two dims of a pair
+#pragma unroll
+            for (int e = 0; e < P; ++e) x[e] *= r * wv[e];
+            if (half) {
+#pragma unroll
+              for (int e = 0; e < P; ++e) {
+                const float up = __shfl_down_sync(0xffffffffu, x[e], ofs & 31);
+                const float dn = __shfl_up_sync(0xffffffffu, x[e], ofs & 31);
+                if (lane * P < 2 * half) x[e] = fmaf(x[e], cs[e], (lane * P < half ? up : dn) * sn[e]);
+              }
+            }
+          }
+        }
+        if (h < 0)
+          store_row_bf16<P>(a.q_out + (t * a.Hq + hh) * D, lane, x);
+        else if (page >= 0)
+          store_page_row<P>(c, layer, page, slot, is_v ? h - c.Hkv : h, is_v, x, lane);
+      }
+    }
   }
 }
 
@@ -573,13 +614,20 @@ int batch_to_dev(const fmoe_paged_batch_t* b, BatchDev* d) {
 }
 
 template <bool NORM>
-static int launch_rows(const PagedDev& c, int layer, const BatchDev& b, const pg::RowsIn& a, cudaStream_t st) {
+static int launch_rows(const PagedDev& c, int layer, const BatchDev& b, pg::RowsIn a, cudaStream_t st) {
   if (b.tokens == 0 || b.n == 0) return FMOE_OK;
+  // A few rows: a head a warp, so that they spread over the SMs (latency).
+  // Many: a warp takes all heads of a row and computes its angles once.
+  const int total = (NORM ? a.Hq : 0) + 2 * c.Hkv, warps = 16 * kNumSMs;
+  a.heads = (int)std::min<int64_t>(total, std::max<int64_t>(1, b.tokens * total / warps));
+  a.chunks = (total + a.heads - 1) / a.heads;
+  const int64_t ctas = (b.tokens * a.chunks + pg::kRowWarps - 1) / pg::kRowWarps;
+  const unsigned grid = (unsigned)std::min<int64_t>(ctas, 4 * kNumSMs);
   ProfScope prof_(NORM ? "paged_rows_kernel<norm>" : "paged_rows_kernel", st);
   if (c.D == 256)
-    pg::paged_rows_kernel<8, NORM><<<(unsigned)b.tokens, 256, 0, st>>>(c, layer, b, a);
+    pg::paged_rows_kernel<8, NORM><<<grid, 32 * pg::kRowWarps, 0, st>>>(c, layer, b, a);
   else
-    pg::paged_rows_kernel<16, NORM><<<(unsigned)b.tokens, 256, 0, st>>>(c, layer, b, a);
+    pg::paged_rows_kernel<16, NORM><<<grid, 32 * pg::kRowWarps, 0, st>>>(c, layer, b, a);
   return check_launch("paged_rows_kernel");
 }
 

@@ -12,7 +12,6 @@
 #include <cmath>
 #include <mutex>
 #include "pattn.cuh"
-#include "tc.cuh"
 
 namespace fmoe {
 namespace pa {
@@ -138,7 +137,7 @@ __device__ __forceinline__ int key_of(int g) {
 template <class C>
 struct Acc {
   float o[C::D / 16][4];
-  float corr[C::BITS == 4 ? C::NG : 1][2];  // 4-bit: sum of P (b + 8 s) - 136 P s of this lane's keys
+  float corr[C::BITS == 4 ? C::NG : 1][2];  // 4-bit: sum of P (b + 8 s) of this lane's keys
   float m[2], l[2];
 };
 
@@ -240,6 +239,15 @@ __device__ __forceinline__ void scores(uint32_t kp, const Query<C>& q, int hf, i
   }
 }
 
+// Two codes less 8, as bf16 (exact).  The values' sums run over thousands of
+// keys: with the 128 of the codes' form left in, they would grow to a hundred
+// times the result and lose its low bits.
+__device__ __forceinline__ uint32_t centred(uint32_t w, int sh) {
+  const uint32_t q = nib_pair(w, sh), k = 0x43084308u;  // 136, 136
+  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q), *reinterpret_cast<const __nv_bfloat162*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // Piece hf of O^T += V^T P^T; p: the weights of rows g, g + 8 of the score
 // product and columns 2t, 2t + 1 (bf16: their transposed fragments in b0, b1).
 template <class C>
@@ -281,8 +289,6 @@ __device__ __forceinline__ void add_values(uint32_t vp, uint32_t pairs, int hf, 
         const float z0 = fmaf(8.f, s0, bf16hi(pr[0][e])), z1 = fmaf(8.f, s1, bf16hi(pr[1][e]));
         fma2(x.corr[gr][0], x.corr[gr][1], z0, p[0], p[1]);
         fma2(x.corr[gr][0], x.corr[gr][1], z1, p[2], p[3]);
-        fma2(x.corr[gr][0], x.corr[gr][1], -136.f, bf16lo(ps0), bf16hi(ps0));
-        fma2(x.corr[gr][0], x.corr[gr][1], -136.f, bf16lo(ps1), bf16hi(ps1));
         const uint32_t c0 = transpose8x8(ps0), c1 = transpose8x8(ps1);
         // the pair (key of slot 2t, of 2t + 1) of one dim in one register: even dims
         // of the octet are the low halves' nibbles, odd dims the high halves'
@@ -290,8 +296,7 @@ __device__ __forceinline__ void add_values(uint32_t vp, uint32_t pairs, int hf, 
         const uint32_t x1 = prmt(w[2][e], w[3][e], 0x5410u), y1 = prmt(w[2][e], w[3][e], 0x7632u);
 #pragma unroll
         for (int n = 0; n < 4; ++n)
-          mma16816(x.o[4 * gr + n], nib_pair(x0, 4 * n), nib_pair(y0, 4 * n), nib_pair(x1, 4 * n), nib_pair(y1, 4 * n),
-                   c0, c1);
+          mma16816(x.o[4 * gr + n], centred(x0, 4 * n), centred(y0, 4 * n), centred(x1, 4 * n), centred(y1, 4 * n), c0, c1);
       }
     }
   }
@@ -632,13 +637,13 @@ __global__ void __launch_bounds__(C::NT, 1)
         if constexpr (C::BITS == 16) {
 #pragma unroll
           for (int hf = 0; hf < H; ++hf, ++used) {
-            tc::pwait(&full[used % NP], (used / NP) & 1, failed, ws.status, 501);
+            wait(&full[used % NP], (used / NP) & 1, failed, ws.status, 501);
             scores<C>(smem_u32(ring + (used % NP) * C::PIECE), q, hf, lane, sc);
             __syncwarp();  // every lane has read the piece
             issue();
           }
         } else {
-          tc::pwait(&full[used % NP], (used / NP) & 1, failed, ws.status, 501);
+          wait(&full[used % NP], (used / NP) & 1, failed, ws.status, 501);
           scores<C>(smem_u32(piece), q, 0, lane, sc);
         }
 #pragma unroll
@@ -700,7 +705,7 @@ __global__ void __launch_bounds__(C::NT, 1)
           const uint32_t b0 = transpose8x8(pack_bf16x2(p[0], p[1])), b1 = transpose8x8(pack_bf16x2(p[2], p[3]));
 #pragma unroll
           for (int hf = 0; hf < H; ++hf, ++used) {
-            tc::pwait(&full[used % NP], (used / NP) & 1, failed, ws.status, 502);
+            wait(&full[used % NP], (used / NP) & 1, failed, ws.status, 502);
             uint8_t* vp = ring + (used % NP) * C::PIECE;
             if (!seen) blank(vp);
             add_values<C>(smem_u32(vp), 0u, hf, p, b0, b1, lane, x);

@@ -2,6 +2,7 @@
 #pragma once
 #include "paged.cuh"
 #include "stage.cuh"
+#include "tc.cuh"
 
 namespace fmoe {
 namespace pa {
@@ -19,6 +20,13 @@ struct AttnArgs {
 // on the split kernel, which holds them as the 8 columns of its products.
 constexpr int kFewRows = 8;
 
+// tc::pwait whose common case, a phase that is over, costs a poll.
+static __device__ __noinline__ void wait_long(uint64_t* bar, uint32_t parity, volatile int* failed, int* status, int site) {
+  tc::pwait(bar, parity, failed, status, site);
+}
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* failed, int* status, int site) {
+  if (!tc::try_wait(bar, parity)) wait_long(bar, parity, failed, status, site);
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));

@@ -30,7 +30,6 @@
 #include <cmath>
 #include <mutex>
 #include "pattn.cuh"
-#include "tc.cuh"
 
 namespace fmoe {
 namespace pa {
@@ -122,13 +121,6 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
   return p != 0;
-}
-// tc::pwait whose common case, a phase that is over, costs a poll.
-__device__ __noinline__ void wait_long(uint64_t* bar, uint32_t parity, volatile int* failed, int* status, int site) {
-  tc::pwait(bar, parity, failed, status, site);
-}
-__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* failed, int* status, int site) {
-  if (!tc::try_wait(bar, parity)) wait_long(bar, parity, failed, status, site);
 }
 // Barrier `id` of the two warps that share rows, true if `p` is in any thread.
 __device__ __forceinline__ bool pair_any(bool p, int id) {
