@@ -407,14 +407,15 @@ struct RowsIn {
 
 // A warp takes `heads` of the q | k | v heads of one row of the step at a time,
 // a lane P neighbouring dims of each.  NORM: norms and rotation (append_qkv);
-// otherwise k and v as they are.  Bound by the rows' bytes: four rows are on
+// otherwise k and v as they are.  Bound by the rows' bytes: rows are on
 // their way while one is worked on, and nothing waits for another warp.  The
 // rates of the rotation are computed once per CTA (a thread a rate), a row's
 // cosines and sines once per warp, in registers, for all its heads.
 constexpr int kRowWarps = 8;
 template <int P, bool NORM>
-__global__ void __launch_bounds__(32 * kRowWarps) paged_rows_kernel(PagedDev c, int layer, BatchDev b, RowsIn a) {
-  constexpr int D = 32 * P, V = P / 8;
+__global__ void __launch_bounds__(32 * kRowWarps, P == 8 ? 3 : 2)
+    paged_rows_kernel(PagedDev c, int layer, BatchDev b, RowsIn a) {
+  constexpr int D = 32 * P, V = P / 8, AHEAD = P == 8 ? 4 : 2;
   __shared__ double rate[NORM ? D / 2 : 1];  // turns per position
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = a.rope / 2;
   if (NORM) {
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) paged_rows_kernel(PagedDev c, 
   const int total = (NORM ? a.Hq : 0) + 2 * c.Hkv;
   const int64_t work = b.tokens * a.chunks;
   int64_t held = -1;  // the row whose angles the lane holds
-  float cs[NORM ? P : 1], sn[NORM ? P : 1];
+  float cs[P], sn[P];
   for (int64_t wi = (int64_t)blockIdx.x * kRowWarps + warp; wi < work; wi += (int64_t)gridDim.x * kRowWarps) {
     const int64_t t = wi / a.chunks;
     const int h0 = (int)(wi - t * a.chunks) * a.heads, h1 = min(h0 + a.heads, total);
@@ -436,14 +437,14 @@ __global__ void __launch_bounds__(32 * kRowWarps) paged_rows_kernel(PagedDev c, 
                    : (is_v && a.v ? a.v + t * a.vs + (int64_t)(h - c.Hkv) * D
                                   : a.k + t * a.ks + (int64_t)(is_v ? h - c.Hkv : h) * D);
     };
-    uint4 raw[4][V];
+    uint4 raw[AHEAD][V];
     auto fetch = [&](int hh, uint4 (&r)[V]) {
       const uint4* p = reinterpret_cast<const uint4*>(source(min(hh, h1 - 1)) + lane * P);
 #pragma unroll
       for (int i = 0; i < V; ++i) r[i] = p[i];
     };
 #pragma unroll
-    for (int u = 0; u < 4; ++u) fetch(h0 + u, raw[u]);
+    for (int u = 0; u < AHEAD; ++u) fetch(h0 + u, raw[u]);
     const int i = seq_of_row(b, t, lane);
     if (i >= b.n) continue;
     const int len = __ldg(b.kv_len + i), pos = len - __ldg(b.q_start + i + 1) + (int)t;
@@ -465,9 +466,13 @@ __global__ void __launch_bounds__(32 * kRowWarps) paged_rows_kernel(PagedDev c, 
         }
       }
     }
-    for (int g0 = h0; g0 < h1; g0 += 4) {
+    // the other dim of a lane's pairs lies in this lane
+    const int ofs = half / P, partner = lane * P < half ? lane + ofs : lane * P < 2 * half ? lane - ofs : lane;
+    float wv[P];
+    bool of_q = false, of_k = false;  // whose weights the lane holds
+    for (int g0 = h0; g0 < h1; g0 += AHEAD) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < AHEAD; ++u) {
         const int hh = g0 + u, h = NORM ? hh - a.Hq : hh;
         if (hh >= h1) break;
         const bool is_v = h >= c.Hkv;
@@ -478,7 +483,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) paged_rows_kernel(PagedDev c, 
           x[8 * i8] = bf16lo(w.x), x[8 * i8 + 1] = bf16hi(w.x), x[8 * i8 + 2] = bf16lo(w.y), x[8 * i8 + 3] = bf16hi(w.y);
           x[8 * i8 + 4] = bf16lo(w.z), x[8 * i8 + 5] = bf16hi(w.z), x[8 * i8 + 6] = bf16lo(w.w), x[8 * i8 + 7] = bf16hi(w.w);
         }
-        fetch(hh + 4, raw[u]);
+        fetch(hh + AHEAD, raw[u]);
         if (NORM) {
           float ss = 0.f;
 #pragma unroll
@@ -490,17 +495,18 @@ __global__ void __launch_bounds__(32 * kRowWarps) paged_rows_kernel(PagedDev c, 
 #pragma unroll
             for (int e = 0; e < P; ++e) x[e] *= r;
           } else {
-            float wv[P];
-            load_row_f32<P>(h < 0 ? a.qn : a.kn, lane, wv);
-            const int ofs = half / P;  // lanes between the two dims of a pair
+            if (!(h < 0 ? of_q : of_k)) {
+              load_row_f32<P>(h < 0 ? a.qn : a.kn, lane, wv);
+              of_q = h < 0;
+              of_k = h >= 0;
+            }
 #pragma unroll
             for (int e = 0; e < P; ++e) x[e] *= r * wv[e];
             if (half) {
 #pragma unroll
               for (int e = 0; e < P; ++e) {
-                const float up = __shfl_down_sync(0xffffffffu, x[e], ofs & 31);
-                const float dn = __shfl_up_sync(0xffffffffu, x[e], ofs & 31);
-                if (lane * P < 2 * half) x[e] = fmaf(x[e], cs[e], (lane * P < half ? up : dn) * sn[e]);
+                const float y = __shfl_sync(0xffffffffu, x[e], partner);
+                if (lane * P < 2 * half) x[e] = fmaf(x[e], cs[e], y * sn[e]);
               }
             }
           }
