@@ -9,10 +9,12 @@
 // from the list that the first one wrote.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include "paged.cuh"
 #include "stage.cuh"
 #include "kvrow.cuh"
 #include "rowops.cuh"
+#include "f32x2.cuh"
 
 namespace fmoe {
 namespace pg {
@@ -383,18 +385,6 @@ __device__ __forceinline__ void store_q4(const float (&v)[P], int lane, uint32_t
   }
 }
 
-template <int P>
-__device__ __forceinline__ void store_page_row(const PagedDev& c, int layer, int page, int slot, int h, int which,
-                                               const float (&v)[P], int lane) {
-  constexpr int D = 32 * P;
-  uint8_t* blk = page_block(c, layer, page, h, which);
-  if (c.bits == 16)
-    store_row_bf16<P>(reinterpret_cast<bf16*>(blk) + (int64_t)slot * D, lane, v);
-  else
-    store_q4<P>(v, lane, reinterpret_cast<uint32_t*>(blk + slot * (D / 2)),
-                reinterpret_cast<uint32_t*>(blk + c.ps * (D / 2) + slot * (D / 16)));
-}
-
 struct RowsIn {
   const bf16 *q, *k, *v, *qn, *kn;
   int64_t qs, ks, vs;  // row strides, values
@@ -407,14 +397,14 @@ struct RowsIn {
 
 // A warp takes `heads` of the q | k | v heads of one row of the step at a time,
 // a lane P neighbouring dims of each.  NORM: norms and rotation (append_qkv);
-// otherwise k and v as they are.  Bound by the rows' bytes: rows are on
+// otherwise k and v as they are.  Bound by the rows' bytes: AHEAD heads are on
 // their way while one is worked on, and nothing waits for another warp.  The
 // rates of the rotation are computed once per CTA (a thread a rate), a row's
 // cosines and sines once per warp, in registers, for all its heads.
 constexpr int kRowWarps = 8;
-template <int P, bool NORM>
+template <int P, int BITS, bool NORM>
 __global__ void __launch_bounds__(32 * kRowWarps, P == 8 ? 3 : 2)
-    paged_rows_kernel(PagedDev c, int layer, BatchDev b, RowsIn a) {
+    paged_rows_kernel(const PagedDev c, int layer, const BatchDev b, const RowsIn a) {
   constexpr int D = 32 * P, V = P / 8, AHEAD = P == 8 ? 4 : 2;
   __shared__ double rate[NORM ? D / 2 : 1];  // turns per position
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = a.rope / 2;
@@ -423,100 +413,131 @@ __global__ void __launch_bounds__(32 * kRowWarps, P == 8 ? 3 : 2)
       rate[j] = exp2(-(double)(2 * j) / a.rope * a.l2t) * 0.15915494309189535;
     __syncthreads();
   }
-  const int total = (NORM ? a.Hq : 0) + 2 * c.Hkv;
+  // the other dim of a lane's pairs lies in this lane
+  const bool turns_here = lane * P < 2 * half;
+  const int ofs = half / P, partner = lane * P < half ? lane + ofs : turns_here ? lane - ofs : lane;
   const int64_t work = b.tokens * a.chunks;
-  int64_t held = -1;  // the row whose angles the lane holds
-  float cs[P], sn[P];
   for (int64_t wi = (int64_t)blockIdx.x * kRowWarps + warp; wi < work; wi += (int64_t)gridDim.x * kRowWarps) {
     const int64_t t = wi / a.chunks;
-    const int h0 = (int)(wi - t * a.chunks) * a.heads, h1 = min(h0 + a.heads, total);
-    auto source = [&](int hh) {
-      const int h = NORM ? hh - a.Hq : hh;
-      const bool is_v = h >= c.Hkv;
-      return h < 0 ? a.q + t * a.qs + (int64_t)hh * D
-                   : (is_v && a.v ? a.v + t * a.vs + (int64_t)(h - c.Hkv) * D
-                                  : a.k + t * a.ks + (int64_t)(is_v ? h - c.Hkv : h) * D);
-    };
-    uint4 raw[AHEAD][V];
-    auto fetch = [&](int hh, uint4 (&r)[V]) {
-      const uint4* p = reinterpret_cast<const uint4*>(source(min(hh, h1 - 1)) + lane * P);
-#pragma unroll
-      for (int i = 0; i < V; ++i) r[i] = p[i];
-    };
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) fetch(h0 + u, raw[u]);
+    const int h0 = (int)(wi - t * a.chunks) * a.heads, h1 = h0 + a.heads, Hq = NORM ? a.Hq : 0;
     const int i = seq_of_row(b, t, lane);
     if (i >= b.n) continue;
     const int len = __ldg(b.kv_len + i), pos = len - __ldg(b.q_start + i + 1) + (int)t;
     const int page = pos >= 0 && pos < len ? page_of(c, __ldg(b.seqs + i), pos >> c.log_ps) : -1;
     const int slot = pos & (c.ps - 1);
-    if (NORM && held != t) {
-      held = t;
+    uint64_t cs[P / 2], sn[P / 2];  // pairs of neighbouring dims
+    if (NORM) {
       // turns reduced in 64 bits: a position of 10^5 times a 32-bit rate is off by
       // a hundredth of a radian
 #pragma unroll
-      for (int e = 0; e < P; ++e) {
-        const int d = lane * P + e;
-        cs[e] = 1.f;
-        sn[e] = 0.f;
-        if (d < 2 * half) {
-          const double turns = pos * rate[d < half ? d : d - half];
-          sincospif(2.0f * (float)(turns - rint(turns)), &sn[e], &cs[e]);
-          if (d < half) sn[e] = -sn[e];  // x cos - up sin, or x cos + dn sin
-        }
-      }
-    }
-    // the other dim of a lane's pairs lies in this lane
-    const int ofs = half / P, partner = lane * P < half ? lane + ofs : lane * P < 2 * half ? lane - ofs : lane;
-    float wv[P];
-    bool of_q = false, of_k = false;  // whose weights the lane holds
-    for (int g0 = h0; g0 < h1; g0 += AHEAD) {
+      for (int e = 0; e < P / 2; ++e) {
+        float co[2] = {1.f, 1.f}, si[2] = {0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int hh = g0 + u, h = NORM ? hh - a.Hq : hh;
-        if (hh >= h1) break;
-        const bool is_v = h >= c.Hkv;
-        float x[P];
-#pragma unroll
-        for (int i8 = 0; i8 < V; ++i8) {
-          const uint4 w = raw[u][i8];
-          x[8 * i8] = bf16lo(w.x), x[8 * i8 + 1] = bf16hi(w.x), x[8 * i8 + 2] = bf16lo(w.y), x[8 * i8 + 3] = bf16hi(w.y);
-          x[8 * i8 + 4] = bf16lo(w.z), x[8 * i8 + 5] = bf16hi(w.z), x[8 * i8 + 6] = bf16lo(w.w), x[8 * i8 + 7] = bf16hi(w.w);
-        }
-        fetch(hh + AHEAD, raw[u]);
-        if (NORM) {
-          float ss = 0.f;
-#pragma unroll
-          for (int e = 0; e < P; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const float r = rsqrtf(ss / (float)D + a.eps);
-          if (is_v) {
-#pragma unroll
-            for (int e = 0; e < P; ++e) x[e] *= r;
-          } else {
-            if (!(h < 0 ? of_q : of_k)) {
-              load_row_f32<P>(h < 0 ? a.qn : a.kn, lane, wv);
-              of_q = h < 0;
-              of_k = h >= 0;
-            }
-#pragma unroll
-            for (int e = 0; e < P; ++e) x[e] *= r * wv[e];
-            if (half) {
-#pragma unroll
-              for (int e = 0; e < P; ++e) {
-                const float y = __shfl_sync(0xffffffffu, x[e], partner);
-                if (lane * P < 2 * half) x[e] = fmaf(x[e], cs[e], y * sn[e]);
-              }
-            }
+        for (int f = 0; f < 2; ++f) {
+          const int d = lane * P + 2 * e + f;
+          if (turns_here) {
+            const double turns = pos * rate[d < half ? d : d - half];
+            sincospif(2.0f * (float)(turns - rint(turns)), &si[f], &co[f]);
+            if (d < half) si[f] = -si[f];  // x cos - y sin, or x cos + y sin, y the pair's other dim
           }
         }
-        if (h < 0)
-          store_row_bf16<P>(a.q_out + (t * a.Hq + hh) * D, lane, x);
-        else if (page >= 0)
-          store_page_row<P>(c, layer, page, slot, is_v ? h - c.Hkv : h, is_v, x, lane);
+        cs[e] = pack2(co[0], co[1]);
+        sn[e] = pack2(si[0], si[1]);
       }
     }
+    // heads [ha, hb) of q (0), k (1) or v (2): src the first one's row, dst where it goes, `apart` bytes to the next
+    auto run = [&](auto kind, int n, const bf16* src, uint8_t* dst, int64_t apart) {
+      constexpr int KIND = decltype(kind)::value;
+      if (n <= 0) return;
+      src += lane * P;
+      uint4 raw[AHEAD][V];
+      auto fetch = [&](int k, uint4 (&r)[V]) {
+        const uint4* p = reinterpret_cast<const uint4*>(src + min(k, n - 1) * D);
+#pragma unroll
+        for (int i8 = 0; i8 < V; ++i8) r[i8] = p[i8];
+      };
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) fetch(u, raw[u]);
+      uint64_t wv[P / 2];
+      if (NORM && KIND < 2) {
+        float w1[P];
+        load_row_f32<P>(KIND ? a.kn : a.qn, lane, w1);
+#pragma unroll
+        for (int e = 0; e < P / 2; ++e) wv[e] = pack2(w1[2 * e], w1[2 * e + 1]);
+      }
+      for (int k0 = 0; k0 < n; k0 += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          if (k0 + u >= n) break;
+          uint4 row[V];
+#pragma unroll
+          for (int i8 = 0; i8 < V; ++i8) row[i8] = raw[u][i8];
+          fetch(k0 + u + AHEAD, raw[u]);
+          if constexpr (NORM || (KIND && BITS == 4)) {
+            uint64_t x[P / 2];
+#pragma unroll
+            for (int i8 = 0; i8 < V; ++i8) {
+              const uint32_t w[4] = {row[i8].x, row[i8].y, row[i8].z, row[i8].w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[4 * i8 + e] = pack2(bf16lo(w[e]), bf16hi(w[e]));
+            }
+            if (NORM) {
+              uint64_t s2 = mul2(x[0], x[0]);
+#pragma unroll
+              for (int e = 1; e < P / 2; ++e) s2 = fma2(x[e], x[e], s2);
+              float ss, s1;
+              unpack2(s2, ss, s1);
+              ss += s1;
+#pragma unroll
+              for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+              const float r = rsqrtf(ss * (1.0f / D) + a.eps);
+              const uint64_t r2 = pack2(r, r);
+#pragma unroll
+              for (int e = 0; e < P / 2; ++e) x[e] = KIND < 2 ? mul2(mul2(x[e], r2), wv[e]) : mul2(x[e], r2);
+              if (KIND < 2 && half) {
+#pragma unroll
+                for (int e = 0; e < P / 2; ++e) {
+                  float x0, x1;
+                  unpack2(x[e], x0, x1);
+                  x0 = __shfl_sync(0xffffffffu, x0, partner);
+                  x1 = __shfl_sync(0xffffffffu, x1, partner);
+                  if (turns_here) x[e] = fma2(x[e], cs[e], mul2(pack2(x0, x1), sn[e]));
+                }
+              }
+            }
+            float v[P];
+#pragma unroll
+            for (int e = 0; e < P / 2; ++e) unpack2(x[e], v[2 * e], v[2 * e + 1]);
+            if constexpr (KIND && BITS == 4) {
+              store_q4<P>(v, lane, reinterpret_cast<uint32_t*>(dst + slot * (D / 2)),
+                          reinterpret_cast<uint32_t*>(dst + c.ps * (D / 2) + slot * (D / 16)));
+            } else {
+#pragma unroll
+              for (int i8 = 0; i8 < V; ++i8)
+                row[i8] = make_uint4(pack_bf16x2(v[8 * i8], v[8 * i8 + 1]), pack_bf16x2(v[8 * i8 + 2], v[8 * i8 + 3]),
+                                     pack_bf16x2(v[8 * i8 + 4], v[8 * i8 + 5]), pack_bf16x2(v[8 * i8 + 6], v[8 * i8 + 7]));
+            }
+          }
+          if constexpr (!(KIND && BITS == 4)) {
+            uint4* o = reinterpret_cast<uint4*>(dst) + lane * V;
+#pragma unroll
+            for (int i8 = 0; i8 < V; ++i8) o[i8] = row[i8];
+          }
+          dst += apart;
+        }
+      }
+    };
+    if (NORM) {
+      const int ha = h0, hb = min(h1, Hq);
+      run(std::integral_constant<int, 0>(), hb - ha, a.q + t * a.qs + (int64_t)ha * D,
+          reinterpret_cast<uint8_t*>(a.q_out + (t * Hq + ha) * D), 2 * D);
+    }
+    if (page < 0) continue;
+    const int64_t at = BITS == 16 ? (int64_t)slot * 2 * D : 0;
+    const int ka = max(h0 - Hq, 0), kb = min(h1 - Hq, c.Hkv), va = max(h0 - Hq - c.Hkv, 0), vb = min(h1 - Hq - c.Hkv, c.Hkv);
+    run(std::integral_constant<int, 1>(), kb - ka, a.k + t * a.ks + (int64_t)ka * D, page_block(c, layer, page, ka, 0) + at, 2 * c.block);
+    run(std::integral_constant<int, 2>(), vb - va, (a.v ? a.v + t * a.vs : a.k + t * a.ks) + (int64_t)va * D,
+        page_block(c, layer, page, va, 1) + at, 2 * c.block);
   }
 }
 
@@ -630,10 +651,9 @@ static int launch_rows(const PagedDev& c, int layer, const BatchDev& b, pg::Rows
   const int64_t ctas = (b.tokens * a.chunks + pg::kRowWarps - 1) / pg::kRowWarps;
   const unsigned grid = (unsigned)std::min<int64_t>(ctas, 4 * kNumSMs);
   ProfScope prof_(NORM ? "paged_rows_kernel<norm>" : "paged_rows_kernel", st);
-  if (c.D == 256)
-    pg::paged_rows_kernel<8, NORM><<<grid, 32 * pg::kRowWarps, 0, st>>>(c, layer, b, a);
-  else
-    pg::paged_rows_kernel<16, NORM><<<grid, 32 * pg::kRowWarps, 0, st>>>(c, layer, b, a);
+  const auto kernel = c.D == 256 ? (c.bits == 16 ? pg::paged_rows_kernel<8, 16, NORM> : pg::paged_rows_kernel<8, 4, NORM>)
+                                 : (c.bits == 16 ? pg::paged_rows_kernel<16, 16, NORM> : pg::paged_rows_kernel<16, 4, NORM>);
+  kernel<<<grid, 32 * pg::kRowWarps, 0, st>>>(c, layer, b, a);
   return check_launch("paged_rows_kernel");
 }
 

@@ -12,6 +12,7 @@
 #include <cmath>
 #include <mutex>
 #include "pattn.cuh"
+#include "f32x2.cuh"
 
 namespace fmoe {
 namespace pa {
@@ -168,12 +169,9 @@ struct Query {
   }
 };
 
-// acc.x += a * b.x, acc.y += a * b.y as one packed operation
-__device__ __forceinline__ void fma2(float& x, float& y, float a, float bx, float by) {
-  asm("{\n .reg .b64 p, q, r;\n mov.b64 p, {%2, %2};\n mov.b64 q, {%3, %4};\n mov.b64 r, {%0, %1};\n"
-      " fma.rn.f32x2 r, p, q, r;\n mov.b64 {%0, %1}, r;\n}\n"
-      : "+f"(x), "+f"(y)
-      : "f"(a), "f"(bx), "f"(by));
+// x += a * bx, y += a * by
+__device__ __forceinline__ void axpy2(float& x, float& y, float a, float bx, float by) {
+  unpack2(fma2(pack2(a, a), pack2(bx, by), pack2(x, y)), x, y);
 }
 
 template <class C>
@@ -231,8 +229,8 @@ __device__ __forceinline__ void scores(uint32_t kp, const Query<C>& q, int hf, i
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float sc = bf16lo(pr[i][e]), bi = fmaf(-128.f, sc, bf16hi(pr[i][e]));
-          fma2(s[2 * i], s[2 * i + 1], bi, q.sum[gr][0], q.sum[gr][1]);
-          fma2(s[2 * i], s[2 * i + 1], sc, acc[2 * i], acc[2 * i + 1]);
+          axpy2(s[2 * i], s[2 * i + 1], bi, q.sum[gr][0], q.sum[gr][1]);
+          axpy2(s[2 * i], s[2 * i + 1], sc, acc[2 * i], acc[2 * i + 1]);
         }
       }
     }
@@ -287,8 +285,8 @@ __device__ __forceinline__ void add_values(uint32_t vp, uint32_t pairs, int hf, 
         const uint32_t ps0 = pack_bf16x2(p[0] * s0, p[1] * s0), ps1 = pack_bf16x2(p[2] * s1, p[3] * s1);
         // v = s (c - 8) + (b + 8 s): only the first part carries the rounding of P s
         const float z0 = fmaf(8.f, s0, bf16hi(pr[0][e])), z1 = fmaf(8.f, s1, bf16hi(pr[1][e]));
-        fma2(x.corr[gr][0], x.corr[gr][1], z0, p[0], p[1]);
-        fma2(x.corr[gr][0], x.corr[gr][1], z1, p[2], p[3]);
+        axpy2(x.corr[gr][0], x.corr[gr][1], z0, p[0], p[1]);
+        axpy2(x.corr[gr][0], x.corr[gr][1], z1, p[2], p[3]);
         const uint32_t c0 = transpose8x8(ps0), c1 = transpose8x8(ps1);
         // the pair (key of slot 2t, of 2t + 1) of one dim in one register: even dims
         // of the octet are the low halves' nibbles, odd dims the high halves'
