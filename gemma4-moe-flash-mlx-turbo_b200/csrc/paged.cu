@@ -465,65 +465,94 @@ __global__ void __launch_bounds__(32 * kRowWarps, P == 8 ? 3 : 2)
 #pragma unroll
         for (int e = 0; e < P / 2; ++e) wv[e] = pack2(w1[2 * e], w1[2 * e + 1]);
       }
+      // two heads at a time: their sums and turns are chains of shuffles, and run side by side
       for (int k0 = 0; k0 < n; k0 += AHEAD) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-          if (k0 + u >= n) break;
-          uint4 row[V];
+        for (int u0 = 0; u0 < AHEAD; u0 += 2) {
+          uint4 row[2][V];
 #pragma unroll
-          for (int i8 = 0; i8 < V; ++i8) row[i8] = raw[u][i8];
-          fetch(k0 + u + AHEAD, raw[u]);
+          for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i8 = 0; i8 < V; ++i8) row[u][i8] = raw[u0 + u][i8];
+            fetch(k0 + u0 + u + AHEAD, raw[u0 + u]);
+          }
+          uint64_t x[2][P / 2];
           if constexpr (NORM || (KIND && BITS == 4)) {
-            uint64_t x[P / 2];
 #pragma unroll
-            for (int i8 = 0; i8 < V; ++i8) {
-              const uint32_t w[4] = {row[i8].x, row[i8].y, row[i8].z, row[i8].w};
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[4 * i8 + e] = pack2(bf16lo(w[e]), bf16hi(w[e]));
+              for (int i8 = 0; i8 < V; ++i8) {
+                const uint32_t w[4] = {row[u][i8].x, row[u][i8].y, row[u][i8].z, row[u][i8].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[u][4 * i8 + e] = pack2(bf16lo(w[e]), bf16hi(w[e]));
+              }
+          }
+          if constexpr (NORM) {
+            float ss[2], s1;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              uint64_t s2 = mul2(x[u][0], x[u][0]);
+#pragma unroll
+              for (int e = 1; e < P / 2; ++e) s2 = fma2(x[u][e], x[u][e], s2);
+              unpack2(s2, ss[u], s1);
+              ss[u] += s1;
             }
-            if (NORM) {
-              uint64_t s2 = mul2(x[0], x[0]);
 #pragma unroll
-              for (int e = 1; e < P / 2; ++e) s2 = fma2(x[e], x[e], s2);
-              float ss, s1;
-              unpack2(s2, ss, s1);
-              ss += s1;
+            for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-              for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-              const float r = rsqrtf(ss * (1.0f / D) + a.eps);
+              for (int u = 0; u < 2; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float r = rsqrtf(ss[u] * (1.0f / D) + a.eps);
               const uint64_t r2 = pack2(r, r);
 #pragma unroll
-              for (int e = 0; e < P / 2; ++e) x[e] = KIND < 2 ? mul2(mul2(x[e], r2), wv[e]) : mul2(x[e], r2);
-              if (KIND < 2 && half) {
+              for (int e = 0; e < P / 2; ++e) x[u][e] = KIND < 2 ? mul2(mul2(x[u][e], r2), wv[e]) : mul2(x[u][e], r2);
+            }
+            if (KIND < 2 && half) {
 #pragma unroll
-                for (int e = 0; e < P / 2; ++e) {
+              for (int e = 0; e < P / 2; ++e)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
                   float x0, x1;
-                  unpack2(x[e], x0, x1);
+                  unpack2(x[u][e], x0, x1);
                   x0 = __shfl_sync(0xffffffffu, x0, partner);
                   x1 = __shfl_sync(0xffffffffu, x1, partner);
-                  if (turns_here) x[e] = fma2(x[e], cs[e], mul2(pack2(x0, x1), sn[e]));
+                  if (turns_here) x[u][e] = fma2(x[u][e], cs[e], mul2(pack2(x0, x1), sn[e]));
+                }
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const bool there = k0 + u0 + u < n;
+            if constexpr (KIND && BITS == 4) {
+              float v[P];
+#pragma unroll
+              for (int e = 0; e < P / 2; ++e) unpack2(x[u][e], v[2 * e], v[2 * e + 1]);
+              if (there)
+                store_q4<P>(v, lane, reinterpret_cast<uint32_t*>(dst + slot * (D / 2)),
+                            reinterpret_cast<uint32_t*>(dst + c.ps * (D / 2) + slot * (D / 16)));
+            } else {
+              if constexpr (NORM) {
+#pragma unroll
+                for (int i8 = 0; i8 < V; ++i8) {
+                  uint32_t w[4];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    float x0, x1;
+                    unpack2(x[u][4 * i8 + e], x0, x1);
+                    w[e] = pack_bf16x2(x0, x1);
+                  }
+                  row[u][i8] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
               }
+              uint4* o = reinterpret_cast<uint4*>(dst) + lane * V;
+              if (there)
+#pragma unroll
+                for (int i8 = 0; i8 < V; ++i8) o[i8] = row[u][i8];
             }
-            float v[P];
-#pragma unroll
-            for (int e = 0; e < P / 2; ++e) unpack2(x[e], v[2 * e], v[2 * e + 1]);
-            if constexpr (KIND && BITS == 4) {
-              store_q4<P>(v, lane, reinterpret_cast<uint32_t*>(dst + slot * (D / 2)),
-                          reinterpret_cast<uint32_t*>(dst + c.ps * (D / 2) + slot * (D / 16)));
-            } else {
-#pragma unroll
-              for (int i8 = 0; i8 < V; ++i8)
-                row[i8] = make_uint4(pack_bf16x2(v[8 * i8], v[8 * i8 + 1]), pack_bf16x2(v[8 * i8 + 2], v[8 * i8 + 3]),
-                                     pack_bf16x2(v[8 * i8 + 4], v[8 * i8 + 5]), pack_bf16x2(v[8 * i8 + 6], v[8 * i8 + 7]));
-            }
+            dst += apart;
           }
-          if constexpr (!(KIND && BITS == 4)) {
-            uint4* o = reinterpret_cast<uint4*>(dst) + lane * V;
-#pragma unroll
-            for (int i8 = 0; i8 < V; ++i8) o[i8] = row[i8];
-          }
-          dst += apart;
+          if (k0 + u0 + 2 >= n) break;
         }
       }
     };
