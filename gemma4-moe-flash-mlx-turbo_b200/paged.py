@@ -24,7 +24,7 @@ import ctypes
 
 import torch
 
-from . import _need_cuda, _ptr, _stream, check, lib
+from . import FMOE_OK, _need_cuda, _ptr, _stream, check, lib
 
 
 class PagedKvC(ctypes.Structure):
@@ -49,6 +49,11 @@ class QKNormRopeC(ctypes.Structure):
         ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float),
         ("rope_theta", ctypes.c_float), ("rope_dims", ctypes.c_int32),
     ]
+
+
+# The current stream's handle without the Stream object around it: these calls
+# run several times per layer and step.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _ids(x, device, what):
@@ -96,6 +101,7 @@ class QKNormRope:
         if q_norm.shape != k_norm.shape or q_norm.dim() != 1:
             raise ValueError(f"paged: q_norm {tuple(q_norm.shape)} and k_norm {tuple(k_norm.shape)} [head_dim] expected")
         self.q_norm, self.k_norm = (w.to(torch.bfloat16).contiguous() for w in (q_norm, k_norm))
+        self.dim = self.q_norm.numel()
         self.c = QKNormRopeC(_ptr(self.q_norm), _ptr(self.k_norm), eps, rope_theta, rope_dims)
         self._ref = ctypes.byref(self.c)
 
@@ -146,13 +152,17 @@ class PagedKVCache:
         self.layers, self.kv_heads, self.head_dim = shape.layers, shape.kv_heads, shape.head_dim
         self.page_size, self.bits, self.num_pages = shape.page_size, shape.bits, shape.num_pages
         self.max_seqs, self.max_blocks = shape.max_seqs, shape.max_blocks
-        self.device = pages.device
+        self.device, self._index = pages.device, pages.device.index
         shape.pages, shape.table, shape.lens = _ptr(pages), _ptr(table), _ptr(lens)
         shape.refs, shape.refused = _ptr(refs), _ptr(self.refused)
         self.c = shape
         self._ref = ctypes.byref(self.c)
         self._op_bytes = lib().fmoe_paged_workspace_bytes(self._ref)
-        self._scratch = {}
+        self._scratch, self._attend_bytes = {}, {}
+        self._lib = lib()
+
+    def _stream(self) -> int:
+        return _raw_stream(self._index) if _raw_stream else _stream()
 
     def _ws(self, kind, nbytes, stream):
         """Scratch of one stream, grown when a call needs more; zeroed when allocated."""
@@ -187,7 +197,7 @@ class PagedKVCache:
         if seqs.numel() != new.numel():
             raise ValueError(f"paged: {seqs.numel()} sequences, {new.numel()} counts")
         kv_len = torch.empty(seqs.numel(), dtype=torch.int32, device=self.device)
-        st = _stream()
+        st = self._stream()
         ws = self._ws("op", self._op_bytes, st)
         check(lib().fmoe_paged_reserve(self._ref, _ptr(seqs), _ptr(new), seqs.numel(), _ptr(kv_len), _ptr(ws),
                                        ws.numel(), st))
@@ -203,7 +213,7 @@ class PagedKVCache:
         a, b = _ids(parents, self.device, "parents"), _ids(children, self.device, "children")
         if a.numel() != b.numel():
             raise ValueError(f"paged: {a.numel()} parents, {b.numel()} children")
-        st = _stream()
+        st = self._stream()
         ws = self._ws("op", self._op_bytes, st)
         check(lib().fmoe_paged_fork(self._ref, _ptr(a), _ptr(b), a.numel(), _ptr(ws), ws.numel(), st))
 
@@ -211,18 +221,18 @@ class PagedKVCache:
         """Gives back the sequences' pages."""
         _distinct(seqs, "seqs")
         s = _ids(seqs, self.device, "seqs")
-        check(lib().fmoe_paged_free(self._ref, _ptr(s), s.numel(), _stream()))
+        check(lib().fmoe_paged_free(self._ref, _ptr(s), s.numel(), self._stream()))
 
     def trim(self, seqs, window: int, sinks: int = 0) -> None:
         """Gives back the sequences' pages that no later position sees under the window."""
         _distinct(seqs, "seqs")
         s = _ids(seqs, self.device, "seqs")
-        check(lib().fmoe_paged_trim(self._ref, _ptr(s), s.numel(), window, sinks, _stream()))
+        check(lib().fmoe_paged_trim(self._ref, _ptr(s), s.numel(), window, sinks, self._stream()))
 
     def compact(self) -> torch.Tensor:
         """Moves the live pages to the front of the pool; their number, int32 [1]."""
         live = torch.empty(1, dtype=torch.int32, device=self.device)
-        st = _stream()
+        st = self._stream()
         ws = self._ws("op", self._op_bytes, st)
         check(lib().fmoe_paged_compact(self._ref, _ptr(live), _ptr(ws), ws.numel(), st))
         return live
@@ -235,53 +245,60 @@ class PagedKVCache:
         a, b = _ids(src, self.device, "src"), _ids(dst, self.device, "dst")
         if a.numel() != b.numel():
             raise ValueError(f"paged: {a.numel()} src, {b.numel()} dst")
-        check(lib().fmoe_paged_copy(self._ref, _ptr(a), _ptr(b), a.numel(), _stream()))
+        check(lib().fmoe_paged_copy(self._ref, _ptr(a), _ptr(b), a.numel(), self._stream()))
 
     # -- a step's rows ---------------------------------------------------------
+    # These run once per layer and step, so their checks are few and their lookups kept.
     def _rows(self, x, heads, batch, what):
-        """A step's rows [tokens, heads, head_dim] in bf16 with whole rows together,
-        and how far apart they are."""
+        """A step's rows [tokens, heads, head_dim] as they are (bf16, whole rows
+        together), or a copy that is; with their address and how far apart they are."""
+        shape, D = x.shape, self.head_dim
+        if len(shape) != 3 or shape[0] != batch.tokens or shape[2] != D or (heads and shape[1] != heads):
+            raise ValueError(f"paged: {what} {tuple(shape)}, [{batch.tokens}, {heads or 'heads'}, {D}] expected")
         if not x.is_cuda:
             raise ValueError("fmoe: tensors must live on a CUDA device")
-        D = self.head_dim
-        if x.dim() != 3 or x.shape[0] != batch.tokens or x.shape[2] != D or (heads and x.shape[1] != heads):
-            raise ValueError(f"paged: {what} {tuple(x.shape)}, [{batch.tokens}, {heads or 'heads'}, {D}] expected")
         if x.dtype != torch.bfloat16:
             x = x.to(torch.bfloat16)
-        if x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != D) or x.stride(0) % 8 or \
-                x.stride(0) < x.shape[1] * D or x.data_ptr() % 16:
+        width = shape[1] * D
+        stride, p = x.stride(), x.data_ptr()
+        if stride[2] != 1 or (stride[1] != D and shape[1] > 1) or stride[0] % 8 or (stride[0] < width and shape[0] > 1) or p % 16:
             x = x.contiguous()
             if x.data_ptr() % 16:
                 x = x.clone()
-        return x, x.stride(0) if x.shape[0] > 1 else x.shape[1] * D
+            return x, x.data_ptr(), width
+        return x, p, stride[0] if shape[0] > 1 else width
+
+    def _out(self, out, q):
+        if out is None:
+            return q.new_empty(q.shape)
+        if out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != q.device:
+            raise ValueError(f"paged: out must be contiguous bf16 {tuple(q.shape)} on {q.device}")
+        return out
 
     def append(self, layer: int, k, v, batch: PagedBatch) -> None:
         """Stores k and v [tokens, kv_heads, head_dim] as they are."""
-        k, ks = self._rows(k, self.kv_heads, batch, "k")
-        v, vs = self._rows(v, self.kv_heads, batch, "v")
-        check(lib().fmoe_paged_append(self._ref, layer, _ptr(k), ks, _ptr(v), vs, batch._ref, _stream()))
+        k, kp, ks = self._rows(k, self.kv_heads, batch, "k")
+        v, vp, vs = self._rows(v, self.kv_heads, batch, "v")
+        rc = self._lib.fmoe_paged_append(self._ref, layer, kp, ks, vp, vs, batch._ref, self._stream())
+        if rc:
+            check(rc)
 
     def append_qkv(self, layer: int, q, k, v, batch: PagedBatch, norm: QKNormRope, out=None) -> torch.Tensor:
         """Norms and turns the projections q [tokens, q_heads, head_dim], k and v
         [tokens, kv_heads, head_dim] (v None: the raw keys), stores k and v and
         returns q."""
-        q, qs = self._rows(q, 0, batch, "q")
-        k, ks = self._rows(k, self.kv_heads, batch, "k")
-        vs = 0
+        q, qp, qs = self._rows(q, 0, batch, "q")
+        k, kp, ks = self._rows(k, self.kv_heads, batch, "k")
+        vp, vs = None, 0
         if v is not None:
-            v, vs = self._rows(v, self.kv_heads, batch, "v")
-        if norm.q_norm.numel() != self.head_dim:
-            raise ValueError(f"paged: norm weights of {norm.q_norm.numel()} values, head_dim {self.head_dim}")
+            v, vp, vs = self._rows(v, self.kv_heads, batch, "v")
+        if norm.dim != self.head_dim:
+            raise ValueError(f"paged: norm weights of {norm.dim} values, head_dim {self.head_dim}")
         out = self._out(out, q)
-        check(lib().fmoe_paged_append_qkv(self._ref, layer, _ptr(q), qs, q.shape[1], _ptr(k), ks, _ptr(v), vs,
-                                          batch._ref, norm._ref, _ptr(out), _stream()))
-        return out
-
-    def _out(self, out, q):
-        if out is None:
-            return torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-        if out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != q.device:
-            raise ValueError(f"paged: out must be contiguous bf16 {tuple(q.shape)} on {q.device}")
+        rc = self._lib.fmoe_paged_append_qkv(self._ref, layer, qp, qs, q.shape[1], kp, ks, vp, vs, batch._ref, norm._ref,
+                                             out.data_ptr(), self._stream())
+        if rc:
+            check(rc)
         return out
 
     def attend(self, layer: int, q, batch: PagedBatch, window: int | None = None, sinks: int = 0, scale: float = 1.0,
@@ -289,12 +306,26 @@ class PagedKVCache:
         """Attention of q [tokens, q_heads, head_dim] over the layer's pages, the
         batch's own rows among them: position p sees j <= p with j > p - window
         (window None or 0: all) or j < sinks.  bf16 [tokens, q_heads, head_dim]."""
-        q, qs = self._rows(q, 0, batch, "q")
+        q, qp, qs = self._rows(q, 0, batch, "q")
         out = self._out(out, q)
         heads = q.shape[1]
-        nbytes = lib().fmoe_paged_attend_workspace_bytes(self._ref, heads, batch.n, batch.tokens, batch.max_new)
-        st = _stream()
+        key = (heads, batch.n, batch.tokens, batch.max_new)
+        nbytes = self._attend_bytes.get(key)
+        if nbytes is None:
+            if len(self._attend_bytes) > 4096:
+                self._attend_bytes.clear()
+            nbytes = self._attend_bytes[key] = self._lib.fmoe_paged_attend_workspace_bytes(self._ref, *key)
+        st = self._stream()
         ws = self._ws("attend", nbytes, st)
-        check(lib().fmoe_paged_attend(self._ref, layer, _ptr(q), qs, heads, batch._ref, window or 0, sinks, scale,
-                                      _ptr(out), _ptr(ws), ws.numel(), st))
+        rc = self._lib.fmoe_paged_attend(self._ref, layer, qp, qs, heads, batch._ref, window or 0, sinks, scale,
+                                         out.data_ptr(), ws.data_ptr(), ws.numel(), st)
+        if rc:
+            check(rc)
         return out
+
+    def status(self) -> int:
+        """Synchronise and read (and clear) whether a device wait of attend's kernels
+        on the current stream gave up."""
+        st = self._stream()
+        ws = self._scratch.get(("attend", st))
+        return FMOE_OK if ws is None else self._lib.fmoe_workspace_status(_ptr(ws), 1, st)
