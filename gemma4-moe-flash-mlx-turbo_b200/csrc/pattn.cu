@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(C::NT, 1)
   extern __shared__ uint8_t sm_raw[];
   __shared__ int2 scan_sh[NW];
   __shared__ int seg_n, failed_sh;
-  __shared__ int tail_sh[2 * NW];
+  __shared__ int tail_sh[2 * NW], list_sh[2 * NW], list_n;
   __shared__ float2 share_sh[2 * NW][8];  // a part's weight in its item's column, and 1 / the column's sum
   __shared__ int64_t item_sh;
   uint8_t* sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
@@ -769,46 +769,50 @@ __global__ void __launch_bounds__(C::NT, 1)
   // -- join the warps' parts: neighbours of one item form a group, [head, tail]
   __syncthreads();
   constexpr int NPART = 2 * NW;
-  if (tid < 8 * NPART) {  // the share of part k in column col; a part without a key of it has no say
-    const int k = tid >> 3, col = tid & 7, item = parts[k].item;
-    const float2 mine = ml[k * 8 + col];
+  if (warp == 0) {  // the parts that there are
+    const bool is = lane < NPART && parts[lane].item >= 0;
+    const uint32_t mask = __ballot_sync(0xffffffffu, is);
+    if (is) list_sh[__popc(mask & ((1u << lane) - 1))] = lane;
+    if (lane == 0) list_n = __popc(mask);
+  }
+  __syncthreads();
+  const int n = list_n;
+  if (tid < 8 * n) {  // the share of a part in column col; a part without a key of it has no say
+    const int at = tid >> 3, k = list_sh[at], col = tid & 7, item = parts[k].item;
     float M = -INFINITY, L = 0.f;
-    bool tail = item >= 0;
-#pragma unroll
-    for (int e = 0; e < NPART; ++e)
-      if (parts[e].item == item) {
-        M = fmaxf(M, ml[e * 8 + col].x);
-        tail &= e <= k;
+    int last = 0;
+#pragma unroll 1
+    for (int e = 0; e < n; ++e)
+      if (parts[list_sh[e]].item == item) {
+        const float2 y = ml[list_sh[e] * 8 + col];
+        const float mn = fmaxf(M, y.x);
+        if (mn > -INFINITY) L = L * ex2(M - mn) + (y.x > -INFINITY ? y.y * ex2(y.x - mn) : 0.f);
+        M = mn;
+        last = e;
       }
-#pragma unroll
-    for (int e = 0; e < NPART; ++e) {
-      const float2 y = ml[e * 8 + col];
-      if (parts[e].item == item && y.x > -INFINITY) L = fmaf(ex2(y.x - M), y.y, L);
-    }
-    share_sh[k][col] = make_float2(item >= 0 && mine.x > -INFINITY ? ex2(mine.x - M) : 0.f, L == 0.f ? 0.f : 1.f / L);
-    tail_sh[k] = tail;
-    if (tail && parts[k].cf != parts[k].cl) ws.ml[parts[k].slot * 8 + col] = make_float2(M, L);
+    const float mine = ml[k * 8 + col].x;
+    share_sh[at][col] = make_float2(mine > -INFINITY ? ex2(mine - M) : 0.f, L == 0.f ? 0.f : 1.f / L);
+    tail_sh[at] = last == at;
+    if (last == at && parts[k].cf != parts[k].cl) ws.ml[parts[k].slot * 8 + col] = make_float2(M, L);
   }
   __syncthreads();
 #pragma unroll 1
   for (int i = tid; i < C::FRAGS; i += NT) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (int k0 = 0; k0 < NPART; k0 += 8) {
-      float4 o[8];
+    for (int k0 = 0; k0 < n; k0 += 4) {
+      float4 o[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {  // a warp's first part is in scratch, its last one in its ring
-        const int k = k0 + e;
-        o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (parts[k].item >= 0)
-          o[e] = parts[k].in_ring ? reinterpret_cast<const float4*>(sm + (k >> 1) * (NP * C::PIECE))[i]
-                                  : __ldcg(reinterpret_cast<const float4*>(ws.wo) +
-                                           ((int64_t)blockIdx.x * NW + (k >> 1)) * 2 * D + i);
+      for (int e = 0; e < 4; ++e) {  // a warp's first part is in scratch, its last one in its ring
+        const int k = list_sh[min(k0 + e, n - 1)];
+        o[e] = parts[k].in_ring ? *reinterpret_cast<const float4*>(sm + (k >> 1) * (NP * C::PIECE) + i * 16)
+                                : __ldcg(reinterpret_cast<const float4*>(ws.wo) +
+                                         ((int64_t)blockIdx.x * NW + (k >> 1)) * 2 * D + i);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int k = k0 + e;
-        const float2 s0 = share_sh[k][2 * t], s1 = share_sh[k][2 * t + 1];
+      for (int e = 0; e < 4; ++e) {
+        if (k0 + e >= n) break;
+        const float2 s0 = share_sh[k0 + e][2 * t], s1 = share_sh[k0 + e][2 * t + 1];
         if (s0.x != 0.f) {
           v.x = fmaf(s0.x, o[e].x, v.x);
           v.z = fmaf(s0.x, o[e].z, v.z);
@@ -817,8 +821,8 @@ __global__ void __launch_bounds__(C::NT, 1)
           v.y = fmaf(s1.x, o[e].y, v.y);
           v.w = fmaf(s1.x, o[e].w, v.w);
         }
-        if (tail_sh[k]) {
-          finish_group<C>(a, ws, parts[k], i, v, s0.y, s1.y, lane);
+        if (tail_sh[k0 + e]) {
+          finish_group<C>(a, ws, parts[list_sh[k0 + e]], i, v, s0.y, s1.y, lane);
           v = make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
