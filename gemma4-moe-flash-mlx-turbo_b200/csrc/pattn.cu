@@ -30,7 +30,8 @@ namespace pa {
 // warps are joined at the end of the CTA, parts in several CTAs by
 // paged_attn_join_kernel, in the order of the keys: no result depends on who
 // arrives first.  An item's beginning (its query, its first page ids) costs a
-// warp about as long as two granules do, so an item counts for kBegin more.
+// warp as long as several granules do, so an item counts for kBegin more (6: 32
+// ragged decodes at 80 us, 89 at 2, 78 at 8; 64 windowed ones at 104, 102 at 2).
 //
 // One granule, with the 8 columns being the item's (row, head) pairs:
 //   S^T [16 keys x 8]   = K  [16 x D] Q^T    mma m16n8k16, A = K  (ldmatrix)
@@ -46,7 +47,7 @@ namespace pa {
 // V's s goes into the weights, v = s (c - 8) + (b + 8 s), and what does not
 // depend on the dim is summed apart in fp32.
 
-constexpr int kBegin = 2;
+constexpr int kBegin = 6;
 
 template <int D_, int BITS_>
 struct Few {
