@@ -695,11 +695,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         if (!seen) {
           const int n = units + KU * min(j + 2, tiles) + j, sv = n % NU;  // this tile's unit of V
           wait(&full[sv], (n / NU) & 1, failed, ws.status, 609);
-          const int t4 = tid - 128, key = t4 >> 2, jj = j0 + key;  // four threads to a key, a block of 64 dims each
+          const int key = 8 * (warp - 4) + (lane & 7), jj = j0 + key;  // four threads to a key, a block of 64 dims each
           if (!(((here >> (key >> 4)) & 1) && jj < r.hi && (jj >= r.low || jj < a.sinks))) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<uint4*>(sm + sv * kUnit + (t4 & 3) * 8192 + key * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(sm + sv * kUnit + (lane >> 3) * 8192 + key * 128 + (e ^ (lane & 7)) * 16) = make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         }
