@@ -123,15 +123,20 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
   return p != 0;
 }
-// Barrier `id` of the two warps that share rows, true if `p` is in any thread.
-__device__ __forceinline__ bool pair_any(bool p, int id) {
-  uint32_t r;
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&r)[16]) {
   asm volatile(
-      "{\n .reg .pred a, b;\n setp.ne.u32 a, %1, 0;\n barrier.cta.red.or.pred b, %2, 64, a;\n selp.u32 %0, 1, 0, b;\n}\n"
-      : "=r"(r)
-      : "r"((uint32_t)p), "r"(id)
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(
+          addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-  return r != 0;
 }
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(addr), "r"(r[0]),
@@ -354,7 +359,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 8);
+      mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(q_full, 4);
@@ -374,9 +379,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  float* l_sh = reinterpret_cast<float*>(sm + C::OFF_ML);  // [2 items][128] sums, zero between uses
-  float* m_sh = l_sh + 256;                                 // [2 items][128] maxima
-  float* x_sh = m_sh + 256;                                 // [128] between the two threads of a row
+  float2* ml_sh = reinterpret_cast<float2*>(sm + C::OFF_ML);  // [2 sides][128] an item's (maximum, sum)
+  float* x_sh = reinterpret_cast<float*>(ml_sh + 256);        // [128] the maximum in use
   const uint32_t tmem = *tmem_at, tO = tmem, tQ = tmem + 256, tS = tmem + 384;
 
   Walk w;
@@ -402,7 +406,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     w.i = lo;
   }
   if (tid == 0) ws.split[blockIdx.x].rows = 0;
-  if (tid < 256) l_sh[tid] = 0.f;
   __syncthreads();
 
   if (any && warp == 0) {
@@ -591,24 +594,26 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     // the products in flight end before the CTA does (a failure may have left some barrier short)
     if (g > 0) tc::drain_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
   } else if (any && warp >= 4 && warp < 12) {
-    // ---- softmax
+    // ---- softmax: a thread is a row, warps 4..7 of the even tiles, 8..11 of the odd
+    // ones, so that what one tile waits for runs beside the other's arithmetic
     const int row = (warp & 3) * 32 + lane, side = (warp - 4) >> 2;
     const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16;
     const int tok = row / a.share;  // the row's token of the tile
-    int g = 0, units = 0, item = 0;
-    while (w.load(ws)) {
+    const int bar_at = 1 + 2 * (warp & 3);  // the rows' two named barriers: tile g's maximum is decided, by g's parity
+    int g0 = 0, units = 0, item = 0;
+    while (w.load(ws)) {  // (a failure elsewhere ends this too: no wait holds any more)
       const RowTile& r = w.r;
       const int k0 = w.k0, k1 = w.k1, tiles = k1 - k0;
       const int p = r.p0 + min(tok, r.tokens - 1), pl = r.p0 + r.tokens - 1;  // the row's position, the last row's
-      float m = -INFINITY, l = 0.f;  // l: of this side's keys
+      float m = -INFINITY, l = 0.f;  // l: of this side's tiles, to the maximum m
       int entry = -1, entry0 = -64;  // lanes hold the pages of 8 tiles' 16-key granules
       // tiles [ka, kb) are seen whole by every row (those of the first positions are looked at one by one)
       const int shift = r.low_tile - r.ns;
       const int ka = a.window ? max(r.ns, floor_div(pl - a.window, kTile) + 1 - shift) : r.ns;
       const int kb = floor_div(r.p0 + 1, kTile) - shift;
 #pragma unroll 1
-      for (int j = 0; j < tiles; ++j, ++g) {
-        const int k = k0 + j;
+      for (int j = (g0 ^ side) & 1; j < tiles; j += 2) {
+        const int k = k0 + j, g = g0 + j;
         if (k >= entry0 + 8) {
           entry0 = k;
           const int kt = k + (lane >> 2), tile = kt < r.ns ? kt : r.low_tile + kt - r.ns;
@@ -617,73 +622,101 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         const uint32_t here = (__ballot_sync(0xffffffffu, entry >= 0) >> (4 * (k - entry0))) & 15;
         const bool whole = here == 15 && k >= ka && k < kb;
         const int j0 = kTile * (k < r.ns ? k : shift + k);
-        const uint32_t tSj = tS + lane_at + (g & 1) * kTile;
-        wait(&s_full[g & 1], (g >> 1) & 1, failed, ws.status, 607);
+        const uint32_t tSj = tS + lane_at + side * kTile;
+        wait(&s_full[side], (g >> 1) & 1, failed, ws.status, 607);
         tc::tc_fence_after();
-        float s[32];
-        tmem_ld32(tSj + 32 * side, s);
-        tc::tmem_ld_wait();
         // the scale is part of the exponent's fma, except where scores are masked
         // (or it is not positive, and a maximum would not pass through it)
-        float mul = a.sl;
-        if (!whole || !(a.sl > 0.f)) {
-          mul = 1.f;
-          const int jb = j0 + 32 * side;
+        const bool plain = whole && a.sl > 0.f;
+        const float mul = plain ? a.sl : 1.f;
+        auto mask = [&](float (&s)[32], int hf) {
+          const int jb = j0 + 32 * hf;
           uint32_t bits = below(jb, p + 1);
           if (a.window) bits &= ~below(jb, p - a.window + 1) | below(jb, a.sinks);
-          bits &= ((here >> (2 * side)) & 1 ? ~0u : 0xffff0000u) & ((here >> (2 * side)) & 2 ? ~0u : 0x0000ffffu);
+          bits &= ((here >> (2 * hf)) & 1 ? ~0u : 0xffff0000u) & ((here >> (2 * hf)) & 2 ? ~0u : 0x0000ffffu);
           keep(s, bits, a.sl);
+        };
+        auto most = [&](const float (&s)[32]) {
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int i = 4; i < 28; i += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[i + e], s[i + 4 + e]);
+          return fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], max3(s[28], s[29], s[30])), s[31]);
+        };
+        constexpr int HELD = C::BITS == 16 ? 2 : 1;  // halves of the tile in registers
+        float s[HELD][32], best;
+        if constexpr (HELD == 2) {
+          tmem_ld32(tSj, s[0]);
+          tmem_ld32(tSj + 32, s[1]);
+          tc::tmem_ld_wait();
+          if (!plain) mask(s[0], 0), mask(s[1], 1);
+          best = fmaxf(most(s[0]), most(s[1])) * mul;
+        } else {
+          tmem_ld32(tSj, s[0]);
+          tc::tmem_ld_wait();
+          if (!plain) mask(s[0], 0);
+          best = most(s[0]);
+          tmem_ld32(tSj + 32, s[0]);
+          tc::tmem_ld_wait();
+          if (!plain) mask(s[0], 1);
+          best = fmaxf(best, most(s[0])) * mul;
         }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int i = 4; i < 28; i += 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[i + e], s[i + 4 + e]);
-        const float best = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], max3(s[28], s[29], s[30])), s[31]) * mul;
-        if (pair_any(best > m + 8.f, 1 + (warp & 3))) {  // in either warp of these rows
-          if (side) x_sh[row] = best;
-          pair_any(false, 1 + (warp & 3));
-          if (!side) x_sh[row] = fmaxf(fmaxf(m, best), x_sh[row]);
-          pair_any(false, 1 + (warp & 3));
-          const float mn = x_sh[row], f = m == mn ? 1.f : ex2(m - mn);
-          m = mn;
-          l *= f;
-          if (j > 0) {
-            wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, failed, ws.status, 608);
-            tc::tc_fence_after();
+        // the maximum in use goes from tile to tile through shared memory
+        if (g > 0) asm volatile("barrier.cta.sync %0, 64;\n" ::"r"(bar_at + (side ^ 1)) : "memory");
+        const float was = j > 0 ? x_sh[row] : -INFINITY;
+        const bool moves = __any_sync(0xffffffffu, best > was + 8.f);
+        const float now = moves ? fmaxf(was, best) : was;
+        x_sh[row] = now;
+        __syncwarp();
+        asm volatile("barrier.cta.arrive %0, 64;\n" ::"r"(bar_at + side) : "memory");
+        if (m != now) l *= ex2(m - now);
+        m = now;
+        if (moves && j > 0) {
+          const float f = was == now ? 1.f : ex2(was - now);
+          wait(&pv_done[side ^ 1], ((g - 1) >> 1) & 1, failed, ws.status, 608);
+          tc::tc_fence_after();
 #pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-              float v[32];
-              uint32_t u[32];
-              tmem_ld32(tO + lane_at + 128 * side + 32 * i, v);
-              tc::tmem_ld_wait();
+          for (int i = 0; i < 16; ++i) {
+            float v[16];
+            uint32_t u[16];
+            tmem_ld16(tO + lane_at + 16 * i, v);
+            tc::tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(v[e] * f);
-              tmem_st32(tO + lane_at + 128 * side + 32 * i, u);
-            }
+            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(v[e] * f);
+            tmem_st16(tO + lane_at + 16 * i, u);
           }
         }
         const float ref = m == -INFINITY ? 0.f : -m;
-        const uint64_t slope = pack2(mul, mul), shift2 = pack2(ref, ref);
+        const uint64_t slope = pack2(mul, mul), ref2 = pack2(ref, ref);
         uint64_t sum = pack2(0.f, 0.f);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          uint32_t pk[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint64_t e = fma2(pack2(s[16 * hf + 2 * i], s[16 * hf + 2 * i + 1]), slope, shift2);
-            float x, y;
-            if (i % 4 == 3) {
-              ex2_fma(e, x, y);
-            } else {
-              unpack2(e, x, y);
-              x = ex2(x);
-              y = ex2(y);
-            }
-            sum = add2(sum, pack2(x, y));
-            pk[i] = pack_bf16x2(x, y);
+          float(&sh)[32] = s[HELD == 2 ? hf : 0];
+          if constexpr (HELD == 1) {
+            tmem_ld32(tSj + 32 * hf, sh);
+            tc::tmem_ld_wait();
+            if (!plain) mask(sh, hf);
           }
-          tmem_st8(tSj + 32 * side + 8 * hf, pk);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint32_t pk[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint64_t e = fma2(pack2(sh[16 * q + 2 * i], sh[16 * q + 2 * i + 1]), slope, ref2);
+              float x, y;
+              if (i % 4 == 3) {
+                ex2_fma(e, x, y);
+              } else {
+                unpack2(e, x, y);
+                x = ex2(x);
+                y = ex2(y);
+              }
+              sum = add2(sum, pack2(x, y));
+              pk[i] = pack_bf16x2(x, y);
+            }
+            tmem_st8(tSj + 32 * hf + 8 * q, pk);
+          }
         }
         {
           float x, y;
@@ -695,31 +728,32 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         if (!seen) {
           const int n = units + KU * min(j + 2, tiles) + j, sv = n % NU;  // this tile's unit of V
           wait(&full[sv], (n / NU) & 1, failed, ws.status, 609);
-          const int key = 8 * (warp - 4) + (lane & 7), jj = j0 + key;  // four threads to a key, a block of 64 dims each
+          const int key = 16 * (warp & 3) + (lane & 15), jj = j0 + key;  // two threads to a key, two blocks of 64 dims each
           if (!(((here >> (key >> 4)) & 1) && jj < r.hi && (jj >= r.low || jj < a.sinks))) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<uint4*>(sm + sv * kUnit + (lane >> 3) * 8192 + key * 128 + (e ^ (lane & 7)) * 16) = make_uint4(0, 0, 0, 0);
+            for (int e = 0; e < 16; ++e)
+              *reinterpret_cast<uint4*>(sm + sv * kUnit + (2 * (lane >> 4) + (e >> 3)) * 8192 + key * 128 + ((e ^ lane) & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-        }
-        if (j + 1 == tiles) {
-          atomicAdd(&l_sh[(item & 1) * 128 + row], l);  // two addends to zero: their order is the same sum
-          if (side == 0) m_sh[(item & 1) * 128 + row] = m;
         }
         tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&p_full[g & 1]);
-          if (j + 1 == tiles) mbar_arrive(l_full);
-        }
+        if (lane == 0) mbar_arrive(&p_full[side]);
       }
+      // this side's sums, when those of the item before are read
+      if (item > 0) wait(o_free, (item - 1) & 1, failed, ws.status, 616);
+      ml_sh[side * 128 + row] = make_float2(m, l);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(l_full);
       units += (KU + 1) * tiles;
+      g0 += tiles;
       ++item;
       w.next();
-      if (__any_sync(0xffffffffu, *failed)) break;
     }
+    if (g0 > 0 && ((g0 ^ side) & 1) == 0)  // no barrier is left half full
+      asm volatile("barrier.cta.sync %0, 64;\n" ::"r"(bar_at + (side ^ 1)) : "memory");
   } else if (any && warp >= 12 && warp < 16) {
     // ---- edges: a thread is a row
     const int row = (warp & 3) * 32 + lane;
@@ -784,8 +818,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       wait(l_full, item & 1, failed, ws.status, 612);
       wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, failed, ws.status, 610);
       tc::tc_fence_after();
-      const float l = l_sh[(item & 1) * 128 + row], m = m_sh[(item & 1) * 128 + row];
-      l_sh[(item & 1) * 128 + row] = 0.f;  // for the item after the next, whose Q comes later
+      const float2 x0 = ml_sh[row], x1 = ml_sh[128 + row];  // the output is to the larger maximum
+      const float m = fmaxf(x0.x, x1.x);
+      const float l = (x0.y != 0.f ? x0.y * ex2(x0.x - m) : 0.f) + (x1.y != 0.f ? x1.y * ex2(x1.x - m) : 0.f);
       if (cf == cl) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         bf16* o = a.out + ((int64_t)(r.row0 + tok) * a.Hq + h * a.share + col) * D + 256 * half;
