@@ -13,19 +13,33 @@
 //   O  += P_j V_j     A = P_j from tensor memory, over S_j's columns, B = V_j as it lies, MN-major
 // With Q and P in tensor memory an instruction reads only B from shared memory,
 // 64 bytes a clock; from shared memory A alone would ask for all of its 128.
-// The issue order S_{j+1}, O += P_j V_j lets the softmax of a tile run under the
-// products of its neighbours.  Weights are bf16 (their sum is of the unrounded
-// ones); O is rescaled, by the softmax's warps, only when a row's maximum passes
-// the one in use by 2^8.
+// Weights are bf16 (their sum is of the unrounded ones); O is rescaled, by the
+// softmax's warps, only when a row's maximum passes the one in use by 2^8.
 //
 // Warps: 0 copies (TMA, 16..64 rows of 64 dims a box, a box in one page), 1
-// issues the products, 4..11 softmax (two threads to a row, half of a tile's keys
-// each), 12..15 the edges of items: Q in, output out, under the products of the
-// neighbouring items.
+// issues the products, 4..7 and 8..11 the softmax of the even and of the odd
+// tiles (a thread a row), 12..15 the edges of items: Q in, output out, under the
+// products of the neighbouring items.  The issue order is S_0 S_1, then O += P_j
+// V_j, S_{j+2}: P_j goes over S_j, and S_{j+2} over P_j with no wait between them.
 //
 // 4-bit pages: warp 0 copies codes and (scale, bias) pairs as they are, and six
-// more warps (2, 3, 16..19) turn them into the units that the bf16 copies would
-// have been: bf16(scale * code + bias), one rounding, 2^-9 of a value.
+// more warps (2, 3, 16..19) turn them into units like the bf16 copies, but of
+// fp16: values to 2^-12 leave the output as near as its own bf16 allows (1.7e-3 of
+// its norm), where bf16 units would double its error (3.7e-3).  Q and the weights
+// are fp16 with them: a row of Q scaled by a power of two that takes its largest
+// value below 2^15, the weights by 2^7.
+//
+// Measured (16 heads): a 4096-token prompt, 8 kv heads of 256, window 1024, 97 us,
+// 620 TFLOP/s of the pairs seen; 512 dims, 385-token chunks with decodes, 326 us,
+// 535; two 1024-token chunks over 4-bit pages, 271 us, 699.  Of a tile's 1810
+// cycles (256 dims) the products take 1024: a side's softmax (2000) and the two
+// products behind it (1350) follow each other, two sides share them.  With 512
+// dims a tile takes 2410, the products 1800 of them (from shared memory Q's upper
+// half feeds them at two thirds of the rate); with 4-bit pages 2700, which is the
+// unpacking.  Slower, and not kept: a softmax thread to half a row (98, 329 and
+// 274 us), three tiles of scores with half of Q in shared memory and a warp of its
+// own for each product (102, 323 and 286), a warp that looks at the barriers for
+// the issuing one (98, 345 and 306).
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -35,23 +49,23 @@
 namespace fmoe {
 namespace pa {
 
-constexpr int kTile = 64;     // keys of a tile
-constexpr int kTileBegin = 2; // an item's beginning and end, in tiles of its time
+constexpr int kTile = 64;      // keys of a tile
+constexpr int kTileBegin = 2;  // an item's beginning and end, in tiles of its time
 constexpr int kUnpackers = 6;  // warps that turn codes into units
-constexpr int kUnit = 32768;  // bytes of a ring unit: 64 keys x 256 dims
+constexpr int kUnit = 32768;   // bytes of a ring unit: 64 keys x 256 dims
 
 template <int D_, int BITS_>
 struct Tile {
   static constexpr int D = D_, BITS = BITS_, HALVES = D / 256, KU = D / 256;  // KU: units of a K tile
   static constexpr int THREADS = BITS == 16 ? 512 : 640;
   static constexpr int NU = BITS == 16 ? (D == 256 ? 6 : 5) : (D == 256 ? 4 : 3);
-  // 4-bit: a stage is 64 rows of codes, then their pairs; a step 4 rows of it
-  static constexpr int CODES = 32 * D, STAGE = CODES + 4 * D, NS = BITS == 16 ? 0 : D == 256 ? 6 : 3, STEPS = kTile / 4;
+  // 4-bit: a stage is 64 rows of codes, then their pairs; a step 8 rows of it
+  static constexpr int CODES = 32 * D, STAGE = CODES + 4 * D, NS = BITS == 16 ? 0 : D == 256 ? 6 : 3, STEPS = kTile / 8;
   static constexpr int OFF_Q = NU * kUnit;  // dims 256.. of Q, 4 blocks of [128 rows][128 bytes], swizzled
   static constexpr int OFF_STAGE = OFF_Q + (D == 512 ? 65536 : 0);
   static constexpr int OFF_BAR = OFF_STAGE + NS * STAGE;
   static constexpr int OFF_ML = OFF_BAR + 304;
-  static constexpr int SMEM = OFF_ML + 2560;  // the base is 1024-byte aligned, as the swizzle wants it
+  static constexpr int SMEM = OFF_ML + 2560 + (BITS == 4 ? 1024 : 0);  // the base is 1024-byte aligned, as the swizzle wants it
   static_assert(SMEM <= 227 * 1024 - 32, "shared memory");
 };
 
@@ -155,10 +169,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x of two values at or below 8 on the multiply-add pipes, for a share of the
+// 2^x of two values at or below 15 on the multiply-add pipes, for a share of the
 // weights: the special function unit's 4 lanes a clock would take all of a
 // tile's time.  x = n + f with n whole and |f| <= 1/2, 2^f by its Taylor series
-// to the fourth power (off by 4e-5 at most; a weight is rounded to 2^-9), n into
+// to the fourth power (off by 4e-5 at most; a weight is rounded to 2^-9 or 2^-12), n into
 // the exponent.  Below 2^-126: zero, as a masked score's -infinity.
 __device__ __forceinline__ void ex2_fma(uint64_t v, float& x, float& y) {
   float a, b;
@@ -189,7 +203,7 @@ __device__ __forceinline__ void keep(float (&s)[32], uint32_t bits, float sl) {
 __device__ __forceinline__ uint32_t below(int jb, int end) {
   return end <= jb ? 0u : end - jb >= 32 ? ~0u : (1u << (end - jb)) - 1;
 }
-constexpr uint32_t kBMajorMN = 1u << 16;
+constexpr uint32_t kBMajorMN = 1u << 16, kBf16 = 1u << 7 | 1u << 10;  // both operands; without it fp16
 
 __device__ __forceinline__ int64_t scan64(int64_t v, int64_t* sh, int64_t* total) {  // exclusive, 1024 threads
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -312,16 +326,24 @@ struct Walk {
   }
 };
 
-// Eight 4-bit values as bf16: each code's bits go into the mantissa of 128, whose
-// subtraction is exact, and one fma rounds.
-__device__ __forceinline__ uint4 unpack8(uint32_t w, __nv_bfloat162 s, __nv_bfloat162 b) {
-  const uint32_t k = 0x43004300u;  // 128, 128
+// A group's (scale, bias) as fp16 (s, b - 16 s), for values s (16 + c) + (b - 16 s).
+// Past 2000 and 32768, where a value might not fit, these are taken instead.
+__device__ __forceinline__ uint32_t group16(uint32_t pair) {
+  const uint32_t top = 0x470044fau, low = 0xc700c4fau;  // (2000, 32768)
+  __nv_bfloat162 p = __hmin2_nan(*reinterpret_cast<const __nv_bfloat162*>(&pair), *reinterpret_cast<const __nv_bfloat162*>(&top));
+  p = __hmax2_nan(p, *reinterpret_cast<const __nv_bfloat162*>(&low));
+  const float s = __low2float(p);
+  return pack_f16x2(s, fmaf(-16.f, s, __high2float(p)));
+}
+// Eight 4-bit values as fp16: a code's bits in the high end of 16's mantissa are 16
+// + c, and one fma makes the value.  It and b - 16 s are rounded to 2^-12.
+__device__ __forceinline__ uint4 unpack8(uint32_t w, uint32_t group) {
+  const __half2 sb = *reinterpret_cast<const __half2*>(&group), s = __low2half2(sb), b = __high2half2(sb);
   uint32_t r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t q = nib_pair(w, 4 * i);
-    const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q), *reinterpret_cast<const __nv_bfloat162*>(&k));
-    const __nv_bfloat162 v = __hfma2(c, s, b);
+    const uint32_t c = ((i == 0 ? w << 6 : i == 1 ? w << 2 : i == 2 ? w >> 2 : w >> 6) & 0x03c003c0u) | 0x4c004c00u;
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&c), s, b);
     r[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
@@ -381,6 +403,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   tc::tc_fence_after();
   float2* ml_sh = reinterpret_cast<float2*>(sm + C::OFF_ML);  // [2 sides][128] an item's (maximum, sum)
   float* x_sh = reinterpret_cast<float*>(ml_sh + 256);        // [128] the maximum in use
+  float* sl_sh = x_sh + 128;  // 4-bit: [2 items][128] the scale of a row's scores
   const uint32_t tmem = *tmem_at, tO = tmem, tQ = tmem + 256, tS = tmem + 384;
 
   Walk w;
@@ -469,7 +492,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     constexpr int N = C::BITS == 16 ? NU : NS;
     for (int k = max(0, n - N); k < n; ++k) tc::drain_wait(C::BITS == 16 ? &full[k % N] : &st_full[k % N], (k / N) & 1);
   } else if (any && C::BITS == 4 && (warp == 2 || warp == 3 || warp >= 16)) {
-    // ---- 4-bit: stages to units, a step of 4 keys a warp at a time: 8 lanes a key, a lane an octet of its groups
+    // ---- 4-bit: stages to units, a step of 8 keys a warp at a time, twice 4: 8 lanes a key, a
+    // lane an octet of its groups
     if constexpr (C::BITS == 4) {
       const int me = warp < 4 ? warp - 2 : warp - 14, key0 = lane >> 3, oct = lane & 7;
       int n = 0, u = 0;  // stages, units
@@ -484,18 +508,26 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           const uint8_t* st = sm + C::OFF_STAGE + s * C::STAGE;
 #pragma unroll 1
           for (int i = (me + kUnpackers - (n * C::STEPS) % kUnpackers) % kUnpackers; i < C::STEPS; i += kUnpackers) {
-            const int key = 4 * i + key0;
+            uint32_t mine[KU];  // a lane turns one or two of the 8 keys' pairs into fp16, for all
 #pragma unroll
-            for (int hf = 0; hf < KU; ++hf) {  // 256 dims
-              if (v && hf != half) continue;
-              const uint4 codes = lds_u4(st + key * (D / 2) + oct * (D / 16) + hf * 16);
-              const uint4 pairs = lds_u4(st + C::CODES + key * (D / 16) + hf * 16);
-              const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w}, pw[4] = {pairs.x, pairs.y, pairs.z, pairs.w};
-              uint8_t* unit = sm + ((u + (v ? 0 : hf)) % NU) * kUnit + key * 128 + (((oct ^ key) & 7) << 4);
+            for (int x = 0; x < KU; ++x) {
+              const int at = 32 * x + lane;
+              mine[x] = group16(*reinterpret_cast<const uint32_t*>(st + C::CODES + (8 * i + at / (D / 64)) * (D / 16) + at % (D / 64) * 4));
+            }
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 p = *reinterpret_cast<const __nv_bfloat162*>(&pw[e]);
-                *reinterpret_cast<uint4*>(unit + e * 8192) = unpack8(cw[e], __low2bfloat162(p), __high2bfloat162(p));
+            for (int x = 0; x < 2; ++x) {
+              const int key = 8 * i + 4 * x + key0;
+#pragma unroll
+              for (int hf = 0; hf < KU; ++hf) {  // 256 dims
+                if (v && hf != half) continue;
+                const uint4 codes = lds_u4(st + key * (D / 2) + oct * (D / 16) + hf * 16);
+                const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
+                uint8_t* unit = sm + ((u + (v ? 0 : hf)) % NU) * kUnit + key * 128 + (((oct ^ key) & 7) << 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int at = (4 * x + key0) * (D / 64) + 4 * hf + e;
+                  *reinterpret_cast<uint4*>(unit + e * 8192) = unpack8(cw[e], __shfl_sync(0xffffffffu, mine[x * (KU - 1)], at & 31));
+                }
               }
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // generic writes -> tensor-core reads
@@ -524,7 +556,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     // ---- products: the whole warp walks and waits, so that what an instruction
     // takes stays in uniform registers; one lane issues
     const bool lead = elect_one();
-    const uint32_t id_s = tc::idesc_n(kTile), id_o = tc::idesc_n(256) | kBMajorMN;
+    constexpr uint32_t kTypes = C::BITS == 4 ? ~kBf16 : ~0u;
+    const uint32_t id_s = tc::idesc_n(kTile) & kTypes, id_o = (tc::idesc_n(256) & kTypes) | kBMajorMN;
     const uint32_t ring = smem_u32(sm), kd = desc_lo(ring, 1), vd = desc_lo(ring, 8192 >> 4);
     int n = 0, s = 0, ph = 0, g = 0, item = 0;  // units, their slot and phase; tiles, items so far
     auto step = [&]() {
@@ -606,6 +639,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       const int k0 = w.k0, k1 = w.k1, tiles = k1 - k0;
       const int p = r.p0 + min(tok, r.tokens - 1), pl = r.p0 + r.tokens - 1;  // the row's position, the last row's
       float m = -INFINITY, l = 0.f;  // l: of this side's tiles, to the maximum m
+      float sl = a.sl;
       int entry = -1, entry0 = -64;  // lanes hold the pages of 8 tiles' 16-key granules
       // tiles [ka, kb) are seen whole by every row (those of the first positions are looked at one by one)
       const int shift = r.low_tile - r.ns;
@@ -625,16 +659,17 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         const uint32_t tSj = tS + lane_at + side * kTile;
         wait(&s_full[side], (g >> 1) & 1, failed, ws.status, 607);
         tc::tc_fence_after();
+        if (C::BITS == 4) sl = sl_sh[(item & 1) * 128 + row];  // written before the item's Q
         // the scale is part of the exponent's fma, except where scores are masked
         // (or it is not positive, and a maximum would not pass through it)
         const bool plain = whole && a.sl > 0.f;
-        const float mul = plain ? a.sl : 1.f;
+        const float mul = plain ? sl : 1.f;
         auto mask = [&](float (&s)[32], int hf) {
           const int jb = j0 + 32 * hf;
           uint32_t bits = below(jb, p + 1);
           if (a.window) bits &= ~below(jb, p - a.window + 1) | below(jb, a.sinks);
           bits &= ((here >> (2 * hf)) & 1 ? ~0u : 0xffff0000u) & ((here >> (2 * hf)) & 2 ? ~0u : 0x0000ffffu);
-          keep(s, bits, a.sl);
+          keep(s, bits, sl);
         };
         auto most = [&](const float (&s)[32]) {
           float mx[4] = {s[0], s[1], s[2], s[3]};
@@ -687,7 +722,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             tmem_st16(tO + lane_at + 16 * i, u);
           }
         }
-        const float ref = m == -INFINITY ? 0.f : -m;
+        // fp16 weights: larger by 2^7 (and so the sums), up to 2^15, so that small ones keep their bits
+        const float ref = (C::BITS == 4 ? 7.f : 0.f) - (m == -INFINITY ? 0.f : m);
         const uint64_t slope = pack2(mul, mul), ref2 = pack2(ref, ref);
         uint64_t sum = pack2(0.f, 0.f);
 #pragma unroll
@@ -713,7 +749,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 y = ex2(y);
               }
               sum = add2(sum, pack2(x, y));
-              pk[i] = pack_bf16x2(x, y);
+              pk[i] = C::BITS == 4 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
             }
             tmem_st8(tSj + 32 * hf + 8 * q, pk);
           }
@@ -727,6 +763,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         const bool seen = whole || (here == 15 && j0 + kTile - 1 < r.hi && (j0 >= r.low || j0 + kTile - 1 < a.sinks));
         if (!seen) {
           const int n = units + KU * min(j + 2, tiles) + j, sv = n % NU;  // this tile's unit of V
+          // A look at the unit's phase is right once the slot's unit before it has come: K
+          // up to this tile's and V up to the last but one have, as its scores are there;
+          // in a ring of three slots it is the last V.
+          if (NU == 3 && g > 0) wait(&pv_done[side ^ 1], ((g - 1) >> 1) & 1, failed, ws.status, 617);
           wait(&full[sv], (n / NU) & 1, failed, ws.status, 609);
           const int key = 16 * (warp & 3) + (lane & 15), jj = j0 + key;  // two threads to a key, two blocks of 64 dims each
           if (!(((here >> (key >> 4)) & 1) && jj < r.hi && (jj >= r.low || jj < a.sinks))) {
@@ -767,6 +807,24 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 #pragma unroll
       for (int e = 0; e < 16; ++e) q[e] = has ? ldg_u4(p + 8 * e) : make_uint4(0, 0, 0, 0);
     };
+    float up = 1.f;  // 4-bit: what the row of Q is multiplied by, a power of two
+    auto scale_q = [&](int i) {  // item i's: the largest value to [2^14, 2^15)
+      if constexpr (C::BITS == 4) {
+        uint32_t top = 0;
+#pragma unroll 1
+        for (int d = 0; d < D; d += 128) {
+          fetch_q(d);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            top = __vmaxu2(__vmaxu2(top, __vmaxu2(q[e].x & 0x7fff7fffu, q[e].y & 0x7fff7fffu)),
+                           __vmaxu2(q[e].z & 0x7fff7fffu, q[e].w & 0x7fff7fffu));
+        }
+        const int f = min(268 - (int)(max(top & 0xffffu, top >> 16) >> 7), 253);
+        up = __uint_as_float((uint32_t)f << 23);
+        sl_sh[(i & 1) * 128 + row] = a.sl * __uint_as_float((uint32_t)(254 - f) << 23);
+      }
+    };
+    auto q_word = [&](uint32_t x) { return C::BITS == 16 ? x : pack_f16x2(bf16lo(x) * up, bf16hi(x) * up); };
     auto store_q = [&]() {  // fetched dims 0 .. 127 and the others: to tensor memory, past 256 to shared memory
 #pragma unroll 1
       for (int d = 0; d < 256; d += 128) {
@@ -776,7 +834,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           uint32_t r[32];
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            r[4 * e] = q[8 * i + e].x, r[4 * e + 1] = q[8 * i + e].y, r[4 * e + 2] = q[8 * i + e].z, r[4 * e + 3] = q[8 * i + e].w;
+            r[4 * e] = q_word(q[8 * i + e].x), r[4 * e + 1] = q_word(q[8 * i + e].y),
+                  r[4 * e + 2] = q_word(q[8 * i + e].z), r[4 * e + 3] = q_word(q[8 * i + e].w);
           tmem_st32(tQ + lane_at + d / 2 + 32 * i, r);
         }
       }
@@ -786,7 +845,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           fetch_q(256 + d);
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            *reinterpret_cast<uint4*>(sm + C::OFF_Q + (d / 64 + (e >> 3)) * 16384 + row * 128 + (((e ^ row) & 7) << 4)) = q[e];
+            *reinterpret_cast<uint4*>(sm + C::OFF_Q + (d / 64 + (e >> 3)) * 16384 + row * 128 + (((e ^ row) & 7) << 4)) =
+                make_uint4(q_word(q[e].x), q_word(q[e].y), q_word(q[e].z), q_word(q[e].w));
         }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       }
@@ -797,6 +857,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     };
     bool more = w.load(ws);
     if (more) {
+      scale_q(0);
       fetch_q(0);
       store_q();
     }
@@ -810,6 +871,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       w.next();
       more = __all_sync(0xffffffffu, !*failed) && w.load(ws);
       if (more) {
+        scale_q(item + 1);  // (the item before this one, whose place it takes, is out)
         fetch_q(0);
         wait(qk_done, item & 1, failed, ws.status, 611);
         tc::tc_fence_after();
