@@ -158,16 +158,20 @@ class PagedKVCache:
         self.c = shape
         self._ref = ctypes.byref(self.c)
         self._op_bytes = lib().fmoe_paged_workspace_bytes(self._ref)
-        self._scratch, self._attend_bytes = {}, {}
+        self._scratch, self._outgrown, self._attend_bytes = {}, [], {}
         self._lib = lib()
 
     def _stream(self) -> int:
         return _raw_stream(self._index) if _raw_stream else _stream()
 
     def _ws(self, kind, nbytes, stream):
-        """Scratch of one stream, grown when a call needs more; zeroed when allocated."""
+        """Scratch of one stream, grown when a call needs more; zeroed when allocated.
+        What it outgrows stays: a captured graph may hold its address."""
         buf = self._scratch.get((kind, stream))
         if buf is None or buf.numel() < nbytes:
+            if buf is not None:
+                self._outgrown.append(buf)
+                nbytes = -(-nbytes >> 24) << 24  # rarely again
             buf = self._scratch[kind, stream] = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
         return buf
 

@@ -81,6 +81,51 @@ def test_attend_long(fm, dev, bits, dim, kv_heads, heads):
     check_attend(cache, q, batch, 1024, 4, dim ** -0.5)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("dim,kv_heads,heads", [(256, 8, 16), (512, 2, 16)])
+@pytest.mark.parametrize("lens,new", [
+    ([9001, 3, 4500, 700, 1], [1, 1, 4, 700, 1]),
+    ([700], [700]),
+    ([300, 40, 900], [300, 40, 123]),
+    ([64] * 60, [64] * 60),          # items of one and of two key tiles
+    ([65, 129] * 40, [33, 47] * 40),
+])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 3)])
+def test_attend_repeats(fm, dev, bits, dim, kv_heads, heads, lens, new, window, sinks):
+    """Short items and items over several CTAs, again and again: the same bits, no wait given up."""
+    cache, order = pu.blank_cache(fm, dev, lens, kv_heads, dim, 32, bits, seed=1)
+    batch = make_batch(fm, dev, order, lens, new)
+    g = torch.Generator(device=dev).manual_seed(3)
+    q = torch.randn(batch.tokens, heads, dim, generator=g, device=dev).bfloat16()
+    first = check_attend(cache, q, batch, window, sinks, dim ** -0.5)
+    differ = sum(~torch.isfinite(o).all() | (o != first).any()
+                 for o in (cache.attend(0, q, batch, window, sinks, dim ** -0.5) for _ in range(40)))
+    assert int(differ) == 0
+    assert cache.status() == fm.FMOE_OK
+
+
+def test_attend_in_a_graph_outlives_larger_calls(fm, dev):
+    """Scratch that a captured call uses is still there after a call that needed more."""
+    lens = [40, 700]
+    cache, order = pu.blank_cache(fm, dev, lens, 2, 256, 32, 16, seed=4)
+    small, large = make_batch(fm, dev, order, lens, [1, 1]), make_batch(fm, dev, order, lens, [40, 700])
+    g = torch.Generator(device=dev).manual_seed(6)
+    q, ql = (torch.randn(b.tokens, 4, 256, generator=g, device=dev).bfloat16() for b in (small, large))
+    stream, graph, out = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.empty_like(q)
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = cache.attend(0, q, small, scale=0.0625)
+        held = cache._scratch["attend", cache._stream()]
+        with torch.cuda.graph(graph, stream=stream):
+            cache.attend(0, q, small, scale=0.0625, out=out)
+        cache.attend(0, ql, large, scale=0.0625)
+        assert any(x is held for x in list(cache._scratch.values()) + cache._outgrown)
+        del held
+        graph.replay()
+    stream.synchronize()
+    assert torch.equal(out, want)
+
+
 def poison_unseen(cache, order, lens, new, window, sinks):
     """NaN and infinities in every row that no query sees."""
     seen = torch.zeros(cache.num_pages, cache.page_size, dtype=torch.bool)
