@@ -238,6 +238,7 @@ __global__ void __launch_bounds__(1024) paged_attn_plan_kernel(PagedDev c, Batch
   const int tid = threadIdx.x, TT = 128 / a.share;
   const int capacity = c.max_blocks << c.log_ps;
   griddep_launch_dependents();
+  griddep_wait();  // the scratch is the split kernel's before
   int64_t listed = 0, before = 0;
   for (int k0 = 0; k0 < b.n; k0 += 1024) {
     const int k = k0 + tid;
@@ -1032,11 +1033,9 @@ static int launch_tiles_c(const PagedDev& c, const BatchDev& b, const AttnArgs& 
     rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE, "pages");
   }
   if (rc) return rc;
-  {
-    ProfScope prof_("paged_attn_plan_kernel", st);
-    paged_attn_plan_kernel<<<1, 1024, 0, st>>>(c, b, a, w);
-  }
-  if ((rc = check_launch("paged_attn_plan_kernel"))) return rc;
+  if ((rc = launch_pdl("paged_attn_plan_kernel", st, dim3(1), 1024, 0,
+                       [&](cudaLaunchConfig_t* cfg) { cudaLaunchKernelEx(cfg, paged_attn_plan_kernel, c, b, a, w); })))
+    return rc;
   if ((rc = launch_pdl(C::BITS == 16 ? "paged_attn_tile_kernel<bf16>" : "paged_attn_tile_kernel<4-bit>", st, dim3(kNumSMs),
                        C::THREADS, C::SMEM, [&](cudaLaunchConfig_t* cfg) {
                          cudaLaunchKernelEx(cfg, paged_attn_tile_kernel<C>, map, c, a, w);
