@@ -274,7 +274,7 @@ class PagedKVCache:
 
     def _out(self, out, q):
         if out is None:
-            return q.new_empty(q.shape)
+            return torch.empty_like(q)  # (contiguous: whole rows of q lie together)
         if out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != q.device:
             raise ValueError(f"paged: out must be contiguous bf16 {tuple(q.shape)} on {q.device}")
         return out
