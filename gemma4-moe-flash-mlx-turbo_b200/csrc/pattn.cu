@@ -354,7 +354,9 @@ __global__ void __launch_bounds__(C::NT, 1)
   extern __shared__ uint8_t sm_raw[];
   __shared__ int2 scan_sh[NW];
   __shared__ int seg_n, failed_sh;
-  __shared__ int tail_sh[2 * NW], list_sh[2 * NW], list_n;
+  __shared__ int list_sh[2 * NW], list_n;
+  __shared__ int2 group_sh[2 * NW];
+  __shared__ const float4* at_sh[2 * NW];
   __shared__ float2 share_sh[2 * NW][8];  // a part's weight in its item's column, and 1 / the column's sum
   __shared__ int64_t item_sh;
   uint8_t* sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
@@ -770,61 +772,70 @@ __global__ void __launch_bounds__(C::NT, 1)
   // -- join the warps' parts: neighbours of one item form a group, [head, tail]
   __syncthreads();
   constexpr int NPART = 2 * NW;
-  if (warp == 0) {  // the parts that there are
+  if (warp == 0) {  // the parts that there are, and where: in a ring, or (a warp's first) in scratch
     const bool is = lane < NPART && parts[lane].item >= 0;
     const uint32_t mask = __ballot_sync(0xffffffffu, is);
-    if (is) list_sh[__popc(mask & ((1u << lane) - 1))] = lane;
+    if (is) {
+      const int at = __popc(mask & ((1u << lane) - 1)), item = parts[lane].item;
+      list_sh[at] = lane;
+      at_sh[at] = parts[lane].in_ring ? reinterpret_cast<const float4*>(sm + (lane >> 1) * (NP * C::PIECE))
+                                      : reinterpret_cast<const float4*>(ws.wo) + ((int64_t)blockIdx.x * NW + (lane >> 1)) * 2 * D;
+      const uint32_t same = __match_any_sync(mask, item);
+      group_sh[at] = make_int2(__popc(mask & ((1u << (__ffs(same) - 1)) - 1)), at - __popc(same & ((1u << lane) - 1)) + __popc(same));
+    }
     if (lane == 0) list_n = __popc(mask);
   }
   __syncthreads();
   const int n = list_n;
   if (tid < 8 * n) {  // the share of a part in column col; a part without a key of it has no say
-    const int at = tid >> 3, k = list_sh[at], col = tid & 7, item = parts[k].item;
+    const int at = tid >> 3, k = list_sh[at], col = tid & 7;
+    const int2 group = group_sh[at];  // its item's parts [x, y)
     float M = -INFINITY, L = 0.f;
-    int last = 0;
-#pragma unroll 1
-    for (int e = 0; e < n; ++e)
-      if (parts[list_sh[e]].item == item) {
-        const float2 y = ml[list_sh[e] * 8 + col];
-        const float mn = fmaxf(M, y.x);
-        if (mn > -INFINITY) L = L * ex2(M - mn) + (y.x > -INFINITY ? y.y * ex2(y.x - mn) : 0.f);
-        M = mn;
-        last = e;
-      }
+#pragma unroll 4
+    for (int e = group.x; e < group.y; ++e) M = fmaxf(M, ml[list_sh[e] * 8 + col].x);
+#pragma unroll 4
+    for (int e = group.x; e < group.y; ++e) {
+      const float2 y = ml[list_sh[e] * 8 + col];
+      L += y.x > -INFINITY ? y.y * ex2(y.x - M) : 0.f;
+    }
     const float mine = ml[k * 8 + col].x;
     share_sh[at][col] = make_float2(mine > -INFINITY ? ex2(mine - M) : 0.f, L == 0.f ? 0.f : 1.f / L);
-    tail_sh[at] = last == at;
-    if (last == at && parts[k].cf != parts[k].cl) ws.ml[parts[k].slot * 8 + col] = make_float2(M, L);
+    if (at == group.y - 1 && parts[k].cf != parts[k].cl) ws.ml[parts[k].slot * 8 + col] = make_float2(M, L);
   }
   __syncthreads();
-#pragma unroll 1
-  for (int i = tid; i < C::FRAGS; i += NT) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-    for (int k0 = 0; k0 < n; k0 += 4) {
-      float4 o[4];
+  constexpr int FR = (C::FRAGS + NT - 1) / NT;  // fragments of a thread, read side by side
+  float4 v[FR];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {  // a warp's first part is in scratch, its last one in its ring
-        const int k = list_sh[min(k0 + e, n - 1)];
-        o[e] = parts[k].in_ring ? *reinterpret_cast<const float4*>(sm + (k >> 1) * (NP * C::PIECE) + i * 16)
-                                : __ldcg(reinterpret_cast<const float4*>(ws.wo) +
-                                         ((int64_t)blockIdx.x * NW + (k >> 1)) * 2 * D + i);
-      }
+  for (int x = 0; x < FR; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int k0 = 0; k0 < n; k0 += 4) {
+    float4 o[4][FR];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (k0 + e >= n) break;
-        const float2 s0 = share_sh[k0 + e][2 * t], s1 = share_sh[k0 + e][2 * t + 1];
+    for (int e = 0; e < 4; ++e) {
+      const float4* from = at_sh[min(k0 + e, n - 1)];
+#pragma unroll
+      for (int x = 0; x < FR; ++x) o[e][x] = from[min(tid + x * NT, C::FRAGS - 1)];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (k0 + e >= n) break;
+      const float2 s0 = share_sh[k0 + e][2 * t], s1 = share_sh[k0 + e][2 * t + 1];
+#pragma unroll
+      for (int x = 0; x < FR; ++x) {
         if (s0.x != 0.f) {
-          v.x = fmaf(s0.x, o[e].x, v.x);
-          v.z = fmaf(s0.x, o[e].z, v.z);
+          v[x].x = fmaf(s0.x, o[e][x].x, v[x].x);
+          v[x].z = fmaf(s0.x, o[e][x].z, v[x].z);
         }
         if (s1.x != 0.f) {
-          v.y = fmaf(s1.x, o[e].y, v.y);
-          v.w = fmaf(s1.x, o[e].w, v.w);
+          v[x].y = fmaf(s1.x, o[e][x].y, v[x].y);
+          v[x].w = fmaf(s1.x, o[e][x].w, v[x].w);
         }
-        if (tail_sh[k0 + e]) {
-          finish_group<C>(a, ws, parts[list_sh[k0 + e]], i, v, s0.y, s1.y, lane);
-          v = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      if (group_sh[k0 + e].y == k0 + e + 1) {
+#pragma unroll
+        for (int x = 0; x < FR; ++x) {
+          if (tid + x * NT < C::FRAGS) finish_group<C>(a, ws, parts[list_sh[k0 + e]], tid + x * NT, v[x], s0.y, s1.y, lane);
+          v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
     }
