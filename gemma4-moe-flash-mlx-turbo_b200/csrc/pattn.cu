@@ -787,6 +787,17 @@ __global__ void __launch_bounds__(C::NT, 1)
   }
   __syncthreads();
   const int n = list_n;
+  constexpr int FR = (C::FRAGS + NT - 1) / NT, B = 4;  // fragments of a thread; parts read side by side
+  float4 o[B][FR];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int e = 0; e < B; ++e) {
+      const float4* from = at_sh[min(k0 + e, n - 1)];
+#pragma unroll
+      for (int x = 0; x < FR; ++x) o[e][x] = from[min(tid + x * NT, C::FRAGS - 1)];
+    }
+  };
+  if (n > 0) fetch(0);  // under the shares (a stretch of beginnings alone has no part)
   if (tid < 8 * n) {  // the share of a part in column col; a part without a key of it has no say
     const int at = tid >> 3, k = list_sh[at], col = tid & 7;
     const int2 group = group_sh[at];  // its item's parts [x, y)
@@ -803,21 +814,13 @@ __global__ void __launch_bounds__(C::NT, 1)
     if (at == group.y - 1 && parts[k].cf != parts[k].cl) ws.ml[parts[k].slot * 8 + col] = make_float2(M, L);
   }
   __syncthreads();
-  constexpr int FR = (C::FRAGS + NT - 1) / NT;  // fragments of a thread, read side by side
   float4 v[FR];
 #pragma unroll
   for (int x = 0; x < FR; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-  for (int k0 = 0; k0 < n; k0 += 4) {
-    float4 o[4][FR];
+  for (int k0 = 0;;) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float4* from = at_sh[min(k0 + e, n - 1)];
-#pragma unroll
-      for (int x = 0; x < FR; ++x) o[e][x] = from[min(tid + x * NT, C::FRAGS - 1)];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < B; ++e) {
       if (k0 + e >= n) break;
       const float2 s0 = share_sh[k0 + e][2 * t], s1 = share_sh[k0 + e][2 * t + 1];
 #pragma unroll
@@ -839,6 +842,8 @@ __global__ void __launch_bounds__(C::NT, 1)
         }
       }
     }
+    if ((k0 += B) >= n) break;
+    fetch(k0);
   }
   // after a wait that gave up, no copy may land in the memory of a CTA that is gone
   if (*failed)
