@@ -422,7 +422,9 @@ struct RowsIn {
 // otherwise k and v as they are.  Bound by the rows' bytes: AHEAD heads are on
 // their way while one is worked on, and nothing waits for another warp.  The
 // rates of the rotation are computed once per CTA (a thread a rate), a row's
-// cosines and sines once per warp, in registers, for all its heads.
+// cosines and sines once per warp, in registers, for all its heads.  Measured: 5486
+// rows of 16 + 8 + 8 heads of 256, 180 MB, 44 us (4.1 TB/s; a warp a head 102 us); 24
+// rows 6 us, a launch and two dependent reads.
 constexpr int kRowWarps = 8;
 template <int P, int BITS, bool NORM>
 __global__ void __launch_bounds__(32 * kRowWarps, P == 8 ? 3 : 2)

@@ -31,7 +31,14 @@ namespace pa {
 // paged_attn_join_kernel, in the order of the keys: no result depends on who
 // arrives first.  An item's beginning (its query, its first page ids) costs a
 // warp as long as several granules do, so an item counts for kBegin more (6: 32
-// ragged decodes at 80 us, 89 at 2, 78 at 8; 64 windowed ones at 104, 102 at 2).
+// ragged decodes in 76 us, 82 at 2, 74 at 8; 64 windowed ones in 100, 99 at 2; 48
+// long ones of 4 bits in 203, 213 at 2).
+//
+// Measured: 32 ragged decodes over 2 kv heads of 512, 331 MB, 75 us (4.4 TB/s); 64
+// over a window of 1024, 8 heads of 256, 512 MB, 100 us (5.1); of both about 4 us
+// go before the first copy, 2..5 in the CTAs' join and 3 in the other one.  48 long
+// ones over 4-bit pages, 617 MB, 203 us (3.0): 500 instructions a granule and head.
+// One short one takes 12 us, each of its reads waiting for the one before.
 //
 // One granule, with the 8 columns being the item's (row, head) pairs:
 //   S^T [16 keys x 8]   = K  [16 x D] Q^T    mma m16n8k16, A = K  (ldmatrix)
@@ -122,6 +129,11 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 r;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
   return r;
+}
+
+// x / y of what is not negative; most are short, and a division of 64 bits is long.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  return (x | y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
 }
 
 // Which of the granule's keys row g of the score product is (row g + 8: 8
@@ -370,6 +382,7 @@ __global__ void __launch_bounds__(C::NT, 1)
   const int capacity = c.max_blocks << c.log_ps;
 
   griddep_launch_dependents();
+  if (tid == 0) asm volatile("prefetch.tensormap [%0];\n" ::"l"(&map) : "memory");
   if (lane < NP) mbar_init(&full[lane], 1);
   mbar_fence_init();
   if (tid == 0) failed_sh = 0;
@@ -428,7 +441,7 @@ __global__ void __launch_bounds__(C::NT, 1)
   int64_t line = m0.sum_u;
   for (int k0 = NT; k0 < b.n; k0 += NT) line += survey(k0).sum_u;
   line *= c.Hkv;
-  const int64_t part = max((int64_t)NW, (line + gridDim.x - 1) / gridDim.x);
+  const int64_t part = max((int64_t)NW, quotient(line + gridDim.x - 1, gridDim.x));
   const int64_t u0 = min(line, blockIdx.x * part), u1 = min(line, u0 + part);
   if (u0 >= u1) {
     if (tid == 0) ws.split[blockIdx.x].rows = 0;
@@ -451,7 +464,7 @@ __global__ void __launch_bounds__(C::NT, 1)
         const Mine m = chunk(k0);
         const int64_t U = base + (int64_t)m.at_u * c.Hkv;
         if (m.ng > 0 && U <= u0 && u0 < U + (int64_t)m.ng * c.Hkv)
-          item_sh = (items + m.at_i) * c.Hkv + (u0 - U) / m.ng;
+          item_sh = (items + m.at_i) * c.Hkv + quotient(u0 - U, m.ng);
         base += (int64_t)m.sum_u * c.Hkv;
         items += m.sum_i;
       }
@@ -480,8 +493,8 @@ __global__ void __launch_bounds__(C::NT, 1)
           s.ns = m.sp.ns;
           s.low_tile = m.sp.low_tile;
           s.item = (int)(item0 + at);
-          s.cf = r0 >= u0 && r0 < u1 ? blockIdx.x : (int)(r0 / part);
-          s.cl = r1 <= u1 ? blockIdx.x : (int)((r1 - 1) / part);
+          s.cf = r0 >= u0 && r0 < u1 ? blockIdx.x : (int)quotient(r0, part);
+          s.cl = r1 <= u1 ? blockIdx.x : (int)quotient(r1 - 1, part);
           s.slot = 2 * blockIdx.x + (r0 > u0);
           s.first_slot = 2 * s.cf + (r0 > s.cf * part);
           segs[at] = s;
