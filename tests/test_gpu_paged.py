@@ -256,6 +256,28 @@ def test_attend_large_scores(fm, dev, scale, new):
     check_attend(cache, q, batch, 0, 0, scale)
 
 
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dim,kv_heads,heads", [(256, 2, 4), (512, 1, 8)])
+@pytest.mark.parametrize("size,q_size", [(1500.0, 2.0 ** -60), (2.0 ** -9, 2.0 ** 60), (1.0, 0.0)])
+def test_attend_4bit_values_and_queries_of_any_size(fm, dev, new, dim, kv_heads, heads, size, q_size):
+    """Scales from 2^-9 to 1500 (values to 12000), queries from 2^-60 to 2^60, zeros.
+    Scores of a deviation of 1/2: with values to 2^-12 (three times that for a whole
+    group) a weight is off by 2^-11 of the sum of its score's magnitudes, about 6."""
+    lens = [700, 90]
+    cache, order = pu.blank_cache(fm, dev, lens, kv_heads, dim, 32, 4, seed=9)
+    pairs = pu.q4_pairs(cache)
+    g = torch.Generator(device=dev).manual_seed(7)
+    s = size * (0.5 + 0.5 * torch.rand(pairs.shape[:-1], generator=g, device=dev))
+    pairs[..., 0] = s.bfloat16()
+    pairs[..., 1] = (-7.5 * s).bfloat16()
+    batch = make_batch(fm, dev, order, lens, [new, new])
+    q = (q_size * torch.randn(batch.tokens, heads, dim, generator=g, device=dev)).bfloat16()
+    q[0, 0] = 0
+    scale = 0.5 / (dim ** 0.5 * 4.6 * 0.75 * size * q_size) if q_size else 1.0
+    check_attend(cache, q, batch, 0, 0, scale)
+    check_attend(cache, q, batch, 64, 3, scale)
+
+
 # ---- rows ------------------------------------------------------------------------
 
 
