@@ -32,12 +32,12 @@ namespace pa {
 // arrives first.  An item's beginning (its query, its first page ids) costs a
 // warp as long as several granules do, so an item counts for kBegin more (6: 32
 // ragged decodes in 76 us, 82 at 2, 74 at 8; 64 windowed ones in 100, 99 at 2; 48
-// long ones of 4 bits in 203, 213 at 2).
+// long ones of 4 bits in 202, 213 at 2).
 //
 // Measured: 32 ragged decodes over 2 kv heads of 512, 331 MB, 75 us (4.4 TB/s); 64
 // over a window of 1024, 8 heads of 256, 512 MB, 100 us (5.1); of both about 4 us
 // go before the first copy, 2..5 in the CTAs' join and 3 in the other one.  48 long
-// ones over 4-bit pages, 617 MB, 203 us (3.0): 500 instructions a granule and head.
+// ones over 4-bit pages, 617 MB, 202 us (3.0): 500 instructions a granule and head.
 // One short one takes 12 us, each of its reads waiting for the one before.
 //
 // One granule, with the 8 columns being the item's (row, head) pairs:
@@ -59,9 +59,9 @@ constexpr int kBegin = 6;
 template <int D_, int BITS_>
 struct Few {
   static constexpr int D = D_, BITS = BITS_, NG = D / 64;
-  // 4-bit granules cost more instructions than copies take: twelve warps hide
-  // more of their latency than eight where the registers allow it.
-  static constexpr int NW = D == 256 && BITS == 4 ? 12 : 8, NT = 32 * NW;
+  // (4-bit, 256 dims: twelve warps of 168 registers take 196 us for 48 long decodes
+  // and 17.1 for 4 short ones, eight 202 and 15.4; two granules at a time the same.)
+  static constexpr int NW = 8, NT = 32 * NW;
   // A ring piece is one copy group: bf16 16 keys x 256 dims of K or V (8 KB);
   // 4-bit a whole granule, K's and V's codes and (scale, bias) pairs.  Its boxes
   // are 16 rows of 128 bytes, swizzled.
@@ -69,7 +69,7 @@ struct Few {
   static constexpr int PER = BITS == 16 ? 2 * H : 1;  // pieces of a granule
   static constexpr int CODES = BITS == 16 ? 8192 : 8 * D, PAIRS = BITS == 4 ? D : 0;
   static constexpr int PIECE = BITS == 16 ? CODES : (2 * (CODES + PAIRS) + 1023) / 1024 * 1024;
-  static constexpr int NP = BITS == 16 || D == 256 ? 3 : 2;  // pieces in a warp's ring
+  static constexpr int NP = BITS == 16 ? 3 : 2;        // pieces in a warp's ring
   static constexpr bool QREG = BITS == 16 || D == 256;       // q's fragments in registers, else in shared memory
   static constexpr int MAXSEG = 64;
   static constexpr int OFF_Q = NW * NP * PIECE, OFF_SEG = OFF_Q + (QREG ? 0 : NW * 16 * D);
@@ -907,7 +907,7 @@ size_t carve(void* base, const PagedDev& c, FewWs* w) {
   w->split = k.take<Split>(kNumSMs);
   w->o = k.take<float>((size_t)2 * kNumSMs * 8 * c.D);
   w->ml = k.take<float2>((size_t)2 * kNumSMs * 8);
-  w->wo = k.take<float>((size_t)Few<256, 4>::NW * kNumSMs * 8 * c.D);  // the most warps that a CTA has
+  w->wo = k.take<float>((size_t)Few<256, 16>::NW * kNumSMs * 8 * c.D);
   return align_up(k.off, 256);
 }
 
