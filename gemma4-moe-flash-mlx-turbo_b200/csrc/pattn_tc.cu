@@ -29,18 +29,18 @@
 // are fp16 with them: a row of Q scaled by a power of two that takes its largest
 // value below 2^15, the weights by 2^7.
 //
-// Measured (16 heads): a 4096-token prompt, 8 kv heads of 256, window 1024, 97 us,
-// 620 TFLOP/s of the pairs seen; 512 dims, 385-token chunks with decodes, 324 us,
-// 538; two 1024-token chunks over 4-bit pages, 271 us, 699.  Of a tile's 1810
+// Measured (16 heads): a 4096-token prompt, 8 kv heads of 256, window 1024, 94 us,
+// 642 TFLOP/s of the pairs seen; 512 dims, 385-token chunks with decodes, 317 us,
+// 550; two 1024-token chunks over 4-bit pages, 268 us, 705.  Of a tile's 1810
 // cycles (256 dims) the products take 1024: a side's softmax (2000) and the two
 // products behind it (1350) follow each other, two sides share them.  With 512
 // dims a tile takes 2410, the products 1800 of them (from shared memory Q's upper
 // half feeds them at two thirds of the rate); with 4-bit pages 2700, which is the
 // unpacking.  Over bf16 pages the card's power limit holds the clock near 1.3 GHz
-// meanwhile.  Slower, and not kept: a softmax thread to half a row (98, 329 and
-// 274 us), three tiles of scores with half of Q in shared memory and a warp of its
-// own for each product (102, 323 and 286), a warp that looks at the barriers for
-// the issuing one (98, 345 and 306).
+// meanwhile.  Slower, and not kept (with kTileBegin 2, where this has 97, 324 and
+// 271 us): a softmax thread to half a row (98, 329 and 274), three tiles of scores
+// with half of Q in shared memory and a warp of its own for each product (102, 323
+// and 286), a warp that looks at the barriers for the issuing one (98, 345 and 306).
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -51,7 +51,9 @@ namespace fmoe {
 namespace pa {
 
 constexpr int kTile = 64;      // keys of a tile
-constexpr int kTileBegin = 2;  // an item's beginning and end, in tiles of its time
+// An item's beginning and end, in tiles of its time (1: 103 us for the prompt and
+// 350 for the chunks above, 2: 97 and 322, 3: 94 and 316, 6: 93 and 329).
+constexpr int kTileBegin = 3;
 constexpr int kUnpackers = 6;  // warps that turn codes into units
 constexpr int kUnit = 32768;   // bytes of a ring unit: 64 keys x 256 dims
 
