@@ -51,7 +51,8 @@ class Server:
                  page_size=16, device="cuda", seed=0):
         gen = torch.Generator(device=device).manual_seed(seed)
         self.layers = [Layer(k, device, gen) for k in kinds]
-        self.embedding = fm.QuantizedLinear.from_float(torch.randn(VOCAB, HIDDEN, generator=gen, device=device), bits=8)
+        self.embedding, self.head = (
+            fm.QuantizedLinear.from_float(torch.randn(VOCAB, HIDDEN, generator=gen, device=device), bits=8) for _ in range(2))
         self.caches = {}
         for kind, (kv_heads, dim, *_) in KINDS.items():
             n = sum(x.kind == kind for x in self.layers)
@@ -77,7 +78,7 @@ class Server:
             y = cache.attend(i, q, b, layer.window, layer.sinks, layer.dim ** -0.5)
             x = x + layer.o(y.view(len(flat), -1)).float()
         last = torch.tensor(new, device=x.device).cumsum(0) - 1
-        return self.embedding(torch.nn.functional.rms_norm(x[last], (HIDDEN,)).bfloat16())
+        return self.head(torch.nn.functional.rms_norm(x[last], (HIDDEN,)).bfloat16())
 
     def decode(self, seqs, logits, steps):
         """Greedy; the tokens of every sequence and the logits that follow them."""
